@@ -30,7 +30,7 @@ extern "C" {
 
 #define M3_ABI_VERSION 3
 
-enum m3_dtype { M3_F32 = 0, M3_F16 = 1, M3_BF16 = 2 };
+enum m3_dtype { M3_F32 = 0, M3_F16 = 1, M3_BF16 = 2, M3_U8 = 3 /* reset flags, 4-bit codes */ };
 
 enum m3_status {
   M3_OK = 0,
@@ -171,6 +171,72 @@ typedef struct m3_gemv_args {
 } m3_gemv_args;
 
 int m3_gemv(const m3_gemv_args* args, void* stream);
+
+/*
+ * Elementwise gated linear recurrence, per (batch, channel):
+ *   f_t = sigmoid(forget_t);  h_t = f_t h_{t-1} + (1 - f_t) value_t;  y_t = h_t silu(gate_t)
+ * (y = h without a gate). Where reset_t is set, token t sees h_{t-1} = 0 (a document boundary).
+ *   value, forget, gate [B,L,C]  one dtype (gate optional), any strides
+ *   reset [B,L] bytes (M3_U8), optional;  state [B,C] float32 h_0, optional (zeros)
+ *   y [B,L,C] in that dtype;  out_state [B,C] float32 h_L (may alias state exactly when L = 1)
+ *   carry [B, ceil(L / m3_gated_tile()), C] float32, channels contiguous: the state before each tile
+ *         of m3_gated_tile() tokens, written by the forward when given and read by the backward
+ * Backward (m3_gated_scan_bwd, with the forward's inputs and carry): dy [B,L,C] and dstate [B,C]
+ * float32 (optional, the gradient of out_state) give dvalue, dforget, dgate [B,L,C] and, when given,
+ * dinitial [B,C] float32. The reference has no such recurrence; it stands beside the SSD scan in
+ * stacks that mix the two.
+ */
+typedef struct m3_gated_args {
+  int64_t length;
+  int32_t batch, channels;
+  int32_t device; /* CUDA device ordinal of every tensor and of `stream` (-1: current) */
+  int32_t reserved;
+  m3_tensor value, forget, gate, reset, state;
+  m3_tensor y, out_state, carry;
+  m3_tensor dy, dstate;
+  m3_tensor dvalue, dforget, dgate, dinitial;
+} m3_gated_args;
+
+int m3_gated_tile(void);
+int m3_gated_scan_fwd(const m3_gated_args* args, void* stream);
+int m3_gated_scan_bwd(const m3_gated_args* args, void* stream);
+
+/*
+ * Few-row projection with 4-bit weights: y[r][o] = sum_i x[r][i] s[o][i / group] (q[o][i] - z[o][i / group]).
+ *   x [rows][in_dim], y [rows][out_dim]   one 16-bit dtype
+ *   codes [out_dim][(in_dim + 1) / 2]     bytes (M3_U8), the even column in a byte's low half
+ *   scales, zeros [out_dim][ceil(in_dim / group)]  one float dtype; zeros optional (8 everywhere)
+ * group 32, 64 or 128. Float32 sums, y rounded once. Any strides; rows of 16-byte-aligned contiguous
+ * bytes are the fast layout. No counterpart in the reference, whose projections are 16- or 32-bit.
+ */
+typedef struct m3_w4_args {
+  int64_t out_dim, in_dim;
+  int32_t rows, group;
+  int32_t device; /* CUDA device ordinal of every tensor and of `stream` (-1: current) */
+  int32_t reserved;
+  m3_tensor x, codes, scales, zeros, y;
+} m3_w4_args;
+
+int m3_linear_w4(const m3_w4_args* args, void* stream);
+
+/*
+ * Newton-Schulz orthogonalisation of `count` matrices update [count][rows][cols] (any float dtype
+ * and strides): X_0 = G / |G|_F (0 where G = 0), then `steps` times
+ *   A = X X^T,  X <- a X + (b A + c A A) X      (on the transpose where rows > cols),
+ * coefficient = {a, b, c}; out [count][rows][cols] is X in out's float dtype. The caller passes
+ * workspace: m3_orthogonalize_workspace_bytes(args) bytes, 256-byte aligned. No counterpart in the
+ * reference, which has no optimiser.
+ */
+typedef struct m3_orth_args {
+  int64_t rows, cols;
+  int32_t count, steps;
+  int32_t device; /* CUDA device ordinal of every tensor and of `stream` (-1: current) */
+  float coefficient[3];
+  m3_tensor update, out, workspace;
+} m3_orth_args;
+
+int64_t m3_orthogonalize_workspace_bytes(const m3_orth_args* args);
+int m3_orthogonalize(const m3_orth_args* args, void* stream);
 
 /* Chunked SSD forward. Returns M3_OK or an M3_ERR_* code. */
 int m3_scan_fwd(const m3_scan_args* args, void* stream);

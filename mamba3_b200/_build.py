@@ -24,7 +24,8 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC",
     "--expt-relaxed-constexpr",
 ]
-UNITS = ["capi.cu", "step.cu", "scan_simt.cu", "scan_umma.cu", "noalloc.cu", "norm.cu", "ssd_train.cu", "gemv.cu"]
+UNITS = ["capi.cu", "step.cu", "scan_simt.cu", "scan_umma.cu", "noalloc.cu", "norm.cu", "ssd_train.cu", "gemv.cu",
+         "gated.cu", "w4.cu", "newton.cu"]
 
 
 def sources() -> list[Path]:

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -16,7 +17,7 @@ import torch
 
 _LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libmamba3_b200.so"
 
-M3_F32, M3_F16, M3_BF16 = 0, 1, 2
+M3_F32, M3_F16, M3_BF16, M3_U8 = 0, 1, 2, 3
 _DTYPES = {torch.float32: M3_F32, torch.float16: M3_F16, torch.bfloat16: M3_BF16}
 ABI_VERSION = 3
 
@@ -162,6 +163,13 @@ def load() -> ctypes.CDLL:
         lib.m3_ssd_train_fwd.restype = ctypes.c_int
         lib.m3_ssd_train_bwd.argtypes = [ctypes.POINTER(SSDArgs), ctypes.c_void_p]
         lib.m3_ssd_train_bwd.restype = ctypes.c_int
+        lib.m3_gated_tile.argtypes = []
+        lib.m3_gated_tile.restype = ctypes.c_int
+        for name in ("m3_gated_scan_fwd", "m3_gated_scan_bwd", "m3_linear_w4", "m3_orthogonalize"):
+            getattr(lib, name).argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+            getattr(lib, name).restype = ctypes.c_int
+        lib.m3_orthogonalize_workspace_bytes.argtypes = [ctypes.c_char_p]
+        lib.m3_orthogonalize_workspace_bytes.restype = ctypes.c_int64
         if lib.m3_abi_version() != ABI_VERSION:
             raise RuntimeError("mamba3_b200 library ABI mismatch; rebuild it")
         _lib = lib
@@ -486,3 +494,101 @@ def gemv(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     args.x, args.w, args.y = _desc(x2), _desc(w), _desc(y)
     _check(lib.m3_gemv(ctypes.byref(args), ctypes.c_void_p(torch.cuda.current_stream(x.device).cuda_stream)), lib)
     return y.view(*x.shape[:-1], w.shape[0])
+
+
+# ---- operators whose argument structs are packed in one go -----------------------------------------
+# A decode-time call costs a few microseconds on the GPU, and filling a ctypes struct field by field
+# costs more than that; struct.pack lays the same bytes out in one call. A tensor is its m3_tensor:
+# pointer, dtype | ndim << 32, six strides.
+
+_TENSOR_CODES = {torch.float32: M3_F32, torch.float16: M3_F16, torch.bfloat16: M3_BF16, torch.uint8: M3_U8,
+                 torch.bool: M3_U8}
+_ABSENT = (0,) * 8
+_PAD = {1: (0,) * 5, 2: (0,) * 4, 3: (0,) * 3}
+
+_GATED_FORMAT = struct.Struct("=qiiii" + "8q" * 14)
+_W4_FORMAT = struct.Struct("=qqiiii" + "8q" * 5)
+_ORTH_FORMAT = struct.Struct("=qqiiifff" + "8q" * 3)
+
+
+def _words(t: torch.Tensor | None) -> tuple:
+    if t is None:
+        return _ABSENT
+    n = t.dim()
+    return (t.data_ptr(), _TENSOR_CODES[t.dtype] | n << 32, *t.stride(), *_PAD[n])
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+@torch.compiler.disable
+def gated_scan_forward(value, forget, gate, reset, state, *, y, out_state, carry=None) -> None:
+    """``m3_gated_scan_fwd`` on ``[B, L, C]`` tensors of one CUDA device, into ``y``, ``out_state``
+    and, for a backward pass, ``carry`` (:func:`gated_carry`)."""
+    lib = load()
+    batch, length, channels = value.shape
+    args = _GATED_FORMAT.pack(length, batch, channels, value.device.index, 0, *_words(value), *_words(forget),
+                              *_words(gate), *_words(reset), *_words(state), *_words(y), *_words(out_state),
+                              *_words(carry), *_ABSENT, *_ABSENT, *_ABSENT, *_ABSENT, *_ABSENT, *_ABSENT)
+    rc = lib.m3_gated_scan_fwd(args, _stream(value.device))
+    if rc:
+        _check(rc, lib)
+
+
+def gated_carry(value: torch.Tensor) -> torch.Tensor:
+    """The buffer for the states before each tile that a backward pass reads."""
+    batch, length, channels = value.shape
+    tile = load().m3_gated_tile()
+    return torch.empty(batch, -(-length // tile), channels, device=value.device, dtype=torch.float32)
+
+
+@torch.compiler.disable
+def gated_scan_backward(value, forget, gate, reset, carry, dy, dstate, want_initial: bool):
+    """``m3_gated_scan_bwd``: ``(dvalue, dforget, dgate or None, dinitial or None)``."""
+    lib = load()
+    batch, length, channels = value.shape
+    dvalue = torch.empty(value.shape, device=value.device, dtype=value.dtype)
+    dforget = torch.empty_like(dvalue)
+    dgate = None if gate is None else torch.empty_like(dvalue)
+    dinitial = torch.empty(batch, channels, device=value.device, dtype=torch.float32) if want_initial else None
+    args = _GATED_FORMAT.pack(length, batch, channels, value.device.index, 0, *_words(value), *_words(forget),
+                              *_words(gate), *_words(reset), *_ABSENT, *_ABSENT, *_ABSENT, *_words(carry), *_words(dy),
+                              *_words(dstate), *_words(dvalue), *_words(dforget), *_words(dgate), *_words(dinitial))
+    rc = lib.m3_gated_scan_bwd(args, _stream(value.device))
+    if rc:
+        _check(rc, lib)
+    return dvalue, dforget, dgate, dinitial
+
+
+@torch.compiler.disable
+def linear_w4(x, codes, scales, zeros, group: int) -> torch.Tensor:
+    """``m3_linear_w4`` on the rows of ``x [rows, in_dim]``."""
+    lib = load()
+    rows, in_dim = x.shape
+    out_dim = codes.shape[0]
+    y = torch.empty(rows, out_dim, device=x.device, dtype=x.dtype)
+    args = _W4_FORMAT.pack(out_dim, in_dim, rows, group, x.device.index, 0, *_words(x), *_words(codes), *_words(scales),
+                           *_words(zeros), *_words(y))
+    rc = lib.m3_linear_w4(args, _stream(x.device))
+    if rc:
+        _check(rc, lib)
+    return y
+
+
+@torch.compiler.disable
+def orthogonalize(update: torch.Tensor, steps: int, coefficients, out_dtype: torch.dtype) -> torch.Tensor:
+    """``m3_orthogonalize`` on a stack ``update [count, rows, cols]``."""
+    lib = load()
+    count, rows, cols = update.shape
+    out = torch.empty(update.shape, device=update.device, dtype=out_dtype)
+    sizes = (rows, cols, count, steps, update.device.index, *coefficients)
+    need = lib.m3_orthogonalize_workspace_bytes(_ORTH_FORMAT.pack(*sizes, *_words(update), *_words(out), *_ABSENT))
+    if need < 0:
+        _check(int(-need), lib)
+    workspace = torch.empty(need, device=update.device, dtype=torch.uint8)
+    args = _ORTH_FORMAT.pack(*sizes, *_words(update), *_words(out), *_words(workspace))
+    rc = lib.m3_orthogonalize(args, _stream(update.device))
+    if rc:
+        _check(rc, lib)
+    return out

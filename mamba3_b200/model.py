@@ -43,6 +43,20 @@ def _default_chunk_sizes(mimo_rank: int) -> tuple[int, int]:
     return training, inference
 
 
+def _few_rows(hidden: torch.Tensor, weight: torch.Tensor) -> bool:
+    """Decode-step projections (at most 4 rows, inference) run as a weight stream on m3_gemv."""
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return False
+    return _ext.gemv_eligible(hidden, weight)
+
+
+def _project(layer: nn.Module, hidden: torch.Tensor) -> torch.Tensor:
+    """``layer(hidden)`` of a projection without bias; few rows of an ``nn.Linear`` on m3_gemv."""
+    if isinstance(layer, nn.Linear) and _few_rows(hidden, layer.weight) and not torch.is_autocast_enabled("cuda"):
+        return _ext.gemv(hidden, layer.weight)
+    return layer(hidden)
+
+
 class _RMSNorm(nn.Module):
     def __init__(self, dim: int, eps: float = 1e-5) -> None:
         super().__init__()
@@ -124,6 +138,8 @@ class _Mamba3Mixer(nn.Module):
         cast to the autocast dtype once and the copy reused until the weight changes (same storage and
         version counter), instead of once per autocast region; the product is bit-identical."""
         layer = getattr(self, name)
+        if not isinstance(layer, nn.Linear):  # 4-bit weights (quant.LinearW4)
+            return layer(hidden)
         weight = layer.weight
         if not (hidden.is_cuda and torch.is_autocast_enabled("cuda") and weight.dtype == torch.float32):
             if self._few_row_projection(hidden, weight):
@@ -143,10 +159,7 @@ class _Mamba3Mixer(nn.Module):
 
     @staticmethod
     def _few_row_projection(hidden: torch.Tensor, weight: torch.Tensor) -> bool:
-        """Decode-step projections (at most 4 rows, inference) run as a weight stream on m3_gemv."""
-        if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
-            return False
-        return _ext.gemv_eligible(hidden, weight)
+        return _few_rows(hidden, weight)
 
     def _views(self, projected: torch.Tensor):
         batch, length, _ = projected.shape
@@ -313,6 +326,10 @@ class _Mamba3Mixer(nn.Module):
         tensors.update(y=both[:, :, 0], y_reverse=both[:, :, 1], final_state=state)
         _ext.scan_forward(sizes=sizes, tensors=tensors, reverse="both", **kw)
         ops.LAST_SCAN_DISPATCH = True
+        if not isinstance(self.out_proj, nn.Linear):  # 4-bit weights: one product a direction, blended after
+            output, backward = (self.out_proj(both[:, :, i].flatten(-2)) for i in (0, 1))
+            blend = torch.sigmoid(self.direction_logit).to(output.dtype)
+            return output * blend + backward * (1.0 - blend)
         return F.linear(both.flatten(-3), self._blended_out_weight(both.dtype))
 
     def _blended_out_weight(self, dtype: torch.dtype) -> torch.Tensor:
@@ -379,7 +396,7 @@ class _Mamba3Mixer(nn.Module):
             raise ValueError(f"expected cache shapes {expected}, got {actual}")
         if cache[0].dtype != torch.float32 or cache[1].dtype != torch.float32:
             raise ValueError("phase and SSM cache tensors must be float32")
-        device = self.in_proj.weight.device
+        device = self.dt_bias.device
         if any(t.device != device for t in cache):
             raise ValueError(f"cache tensors must be on {device}")
 
@@ -679,4 +696,4 @@ class _CudaGraphDecoder:
 
     def _parameter_signature(self):
         return tuple((id(p), p._version, p.data_ptr(), p.device, p.dtype, tuple(p.shape))
-                     for p in self.model.parameters())
+                     for p in (*self.model.parameters(), *self.model.buffers()))

@@ -1,0 +1,110 @@
+"""The gated recurrence off the GPU: its PyTorch form against the token-by-token definition, its
+gradient against differences, the module's prefill / step agreement and every refusal."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from _operator_refs import gated_scan64
+from mamba3_b200 import GatedRecurrence, gated_scan, gated_step
+
+
+def _inputs(batch, length, channels, dtype=torch.float64, gate=True, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    make = lambda *shape: torch.randn(*shape, generator=g, dtype=torch.float64)  # noqa: E731
+    value, forget = make(batch, length, channels), make(batch, length, channels) + 2.0
+    return (value.to(dtype), forget.to(dtype), make(batch, length, channels).to(dtype) if gate else None,
+            make(batch, channels))
+
+
+@pytest.mark.parametrize("length", [1, 2, 3, 64, 129])
+@pytest.mark.parametrize("gate", [True, False])
+@pytest.mark.parametrize("with_reset", [True, False])
+def test_torch_form_is_the_recurrence(length, gate, with_reset):
+    value, forget, g, state = _inputs(2, length, 5, gate=gate)
+    reset = torch.rand(2, length, generator=torch.Generator().manual_seed(1)) < 0.2 if with_reset else None
+    y, final = gated_scan(value, forget, g, initial_state=state, reset=reset)
+    want_y, want_final = gated_scan64(value, forget, g, state, reset)
+    torch.testing.assert_close(y, want_y, rtol=1e-12, atol=1e-12)
+    torch.testing.assert_close(final, want_final, rtol=1e-12, atol=1e-12)
+
+
+def test_gradient_against_differences():
+    value, forget, g, state = _inputs(2, 7, 3)
+    reset = torch.zeros(2, 7, dtype=torch.bool)
+    reset[0, 0] = reset[1, 4] = True
+    leaves = [t.requires_grad_() for t in (value, forget, g, state)]
+    assert torch.autograd.gradcheck(lambda v, f, q, s: gated_scan(v, f, q, initial_state=s, reset=reset), leaves)
+
+
+def test_step_continues_a_scan():
+    value, forget, g, state = _inputs(3, 9, 4)
+    y, final = gated_scan(value, forget, g, initial_state=state)
+    for t in range(9):
+        out, state = gated_step(value[:, t], forget[:, t], state, g[:, t])
+        torch.testing.assert_close(out, y[:, t], rtol=1e-12, atol=1e-12)
+    torch.testing.assert_close(state, final, rtol=1e-12, atol=1e-12)
+
+
+@pytest.mark.parametrize("shape", [(0, 4, 3), (2, 0, 3), (2, 4, 0)])
+def test_empty_inputs(shape):
+    value = torch.empty(shape)
+    state = torch.randn(shape[0], shape[2])
+    y, final = gated_scan(value, value, value, initial_state=state)
+    assert y.shape == shape
+    torch.testing.assert_close(final, state)
+    assert gated_scan(value, value)[1].shape == state.shape
+
+
+def test_refusals():
+    v = torch.randn(2, 4, 3)
+    with pytest.raises(ValueError, match=r"\[B, L, C\]"):
+        gated_scan(v[0], v[0])
+    with pytest.raises(ValueError, match="match value's shape"):
+        gated_scan(v, v[:, :3])
+    with pytest.raises(ValueError, match="match value's shape"):
+        gated_scan(v, v, v[:, :, :2])
+    with pytest.raises(ValueError, match="same dtype"):
+        gated_scan(v, v.double())
+    with pytest.raises(ValueError, match="state must have shape"):
+        gated_scan(v, v, initial_state=torch.zeros(3, 2))
+    with pytest.raises(ValueError, match="reset must have shape"):
+        gated_scan(v, v, reset=torch.zeros(2, 3, dtype=torch.bool))
+    with pytest.raises(ValueError, match="reset must be bool"):
+        gated_scan(v, v, reset=torch.zeros(2, 4))
+    with pytest.raises(ValueError, match=r"\[B, C\]"):
+        gated_step(v, v, torch.zeros(2, 3))
+    with pytest.raises(ValueError, match="needs a state"):
+        gated_step(v[:, 0], v[:, 0], None)
+    with pytest.raises(ValueError, match="out_state must be float32"):
+        gated_step(v[:, 0], v[:, 0], torch.zeros(2, 3), out_state=torch.zeros(2, 4))
+
+
+def test_module_prefill_then_step_is_forward():
+    torch.manual_seed(0)
+    model = GatedRecurrence(32, depth=2).double().eval()
+    x = torch.randn(2, 12, 32, dtype=torch.float64)
+    with torch.no_grad():
+        full = model(x)
+        out, cache = model.prefill(x[:, :8])
+        torch.testing.assert_close(out, full[:, :8], rtol=1e-9, atol=1e-9)
+        for t in range(8, 12):
+            out, cache = model.step(x[:, t:t + 1], cache)
+            torch.testing.assert_close(out, full[:, t:t + 1], rtol=1e-9, atol=1e-9)
+
+
+def test_module_refusals():
+    with pytest.raises(ValueError, match="d_model"):
+        GatedRecurrence(0)
+    with pytest.raises(ValueError, match="depth"):
+        GatedRecurrence(8, depth=0)
+    model = GatedRecurrence(8, depth=1)
+    with pytest.raises(ValueError, match="expected"):
+        model(torch.randn(2, 3, 9))
+    with pytest.raises(ValueError, match="non-empty"):
+        model.prefill(torch.randn(2, 0, 8))
+    with pytest.raises(ValueError, match=r"\[batch, 1, 8\]"):
+        model.step(torch.randn(2, 2, 8))
+    with pytest.raises(ValueError, match="cache for 1 layers"):
+        model.step(torch.randn(2, 1, 8), [])
