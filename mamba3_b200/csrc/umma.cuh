@@ -95,7 +95,7 @@ __device__ __forceinline__ uint64_t global_ns() {
 
 // Bounded wait for mbarrier phase `parity`; false (and the device error word set) on timeout.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-  const uint64_t start = global_ns();
+  uint64_t start = 0;  // taken only once a wait turns out long: reading the timer costs more than a ready wait
   for (uint32_t i = 0;; ++i) {
     uint32_t done;
     asm volatile(
@@ -105,9 +105,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
         : "r"(bar), "r"(parity)
         : "memory");
     if (done) return true;
-    if ((i & 255u) == 255u && global_ns() - start > 2000000000ull) {
-      atomicExch(&g_device_error, kErrMbarTimeout);
-      return false;
+    if ((i & 255u) == 255u) {
+      if (start == 0) {
+        start = global_ns();
+      } else if (global_ns() - start > 2000000000ull) {
+        atomicExch(&g_device_error, kErrMbarTimeout);
+        return false;
+      }
     }
   }
 }
