@@ -20,31 +20,53 @@ namespace m3 {
 
 int report_error(int code, const char* msg);
 
+// The error word of this unit's bounded waits, for m3_device_error(); the device is synchronised.
+int read_gated_error(int clear) {
+  int host = 0;
+  if (cudaMemcpyFromSymbol(&host, g_device_error, sizeof(int)) != cudaSuccess) return -1;
+  if (clear) {
+    const int zero = 0;
+    if (cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int)) != cudaSuccess) return -1;
+  }
+  return host;
+}
+
 namespace {
 
-constexpr int kTile = 64;      // tokens a tile: the training forward keeps the state before each
-constexpr int kChannels = 64;  // channels a CTA
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
-constexpr int kRun = kTile / kWarps;  // consecutive tokens of a thread; it has two neighbouring channels
-constexpr float kFloor = 1e-37f;      // least product of decays without a reset: see fold()
+using umma::mbar_expect_tx;
+using umma::mbar_wait;
+using umma::smem_u32;
+using umma::tma_load3;
+
+constexpr int kTile = 64;        // tokens a tile: the training forward keeps the state before each
+constexpr int kChannels = 64;    // channels a CTA; a thread has two neighbouring ones
+constexpr float kFloor = 1e-37f; // least product of decays without a reset: see fold()
+
+// exp2 and reciprocal of the special-function unit, results below 2^-126 taken as 0. The compiler's __expf and
+// __fdividef add the handling of such values, which no use here can tell apart.
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // f = sigmoid(x) and 1 - f = sigmoid(-x), both to a few units in the last place; x below -80 is taken as -80
 // (f = 2e-35), so that exp stays finite; NaN stays NaN.
 __device__ __forceinline__ void keep_lose(float x, float& keep, float& lose) {
   float c;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(x), "f"(-80.0f));
-  const float e = __expf(-c);
-  keep = __fdividef(1.0f, 1.0f + e);
+  const float e = ex2_approx(c * -kLog2e);
+  keep = rcp_approx(1.0f + e);
   lose = e * keep;
 }
 
-__device__ __forceinline__ float sigmoid_approx(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+__device__ __forceinline__ float sigmoid_approx(float x) { return rcp_approx(1.0f + ex2_approx(x * -kLog2e)); }
 
 // A run of tokens as a map of the state before it: h -> a h + h0. a is exactly 0 where a reset lies in the run,
 // and then nothing of h passes, not even an infinity or NaN; otherwise a product of decays is kept at kFloor or
 // more, so that an infinity or NaN before the run does pass.
 __device__ __forceinline__ float fold(float a, float h0, float h) { return a == 0.0f ? h0 : fmaf(a, h, h0); }
+__device__ __forceinline__ float2 fold(float4 m, float2 h) { return make_float2(fold(m.x, m.z, h.x), fold(m.y, m.w, h.y)); }
 
 // ---- two neighbouring values ---------------------------------------------------------------------
 
@@ -67,53 +89,46 @@ template <> struct Two<__nv_bfloat16> {
 
 // ---- tiles ---------------------------------------------------------------------------------------
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {  // zeros where it is not there
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// Start copying tokens t0 .. t0 + 63 of channels c0 .. c0 + 63 to a tile [64][64]; what is outside reads as 0.
-template <typename T, bool kVec>
+// Tokens t0 .. t0 + 63 of channels c0 .. c0 + 63 to a tile [64][64], for inputs that TMA cannot read: any
+// strides; what is outside reads as 0.
+template <typename T, int kThreads>
 __device__ __forceinline__ void load_tile(T* tile, const m3_tensor& from, int b, int64_t t0, int c0, int64_t length, int channels) {
   const T* base = static_cast<const T*>(from.data) + b * from.stride[0];
-  if constexpr (kVec) {  // 16-byte words of a token's channels, each inside or outside as a whole
-    constexpr int kWord = 16 / sizeof(T), kRow = kChannels / kWord;
-    const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(tile));
-#pragma unroll
-    for (int i = threadIdx.x; i < kTile * kRow; i += kThreads) {
-      const int t = i / kRow, c = i % kRow * kWord;
-      const bool there = t0 + t < length && c0 + c < channels;
-      copy16(to + (t * kChannels + c) * sizeof(T), there ? base + (t0 + t) * from.stride[1] + c0 + c : base, there);
-    }
-  } else {
 #pragma unroll 8
-    for (int i = threadIdx.x; i < kTile * kChannels; i += kThreads) {
-      const int t = i / kChannels, c = i % kChannels;
-      tile[i] = t0 + t < length && c0 + c < channels ? base[(t0 + t) * from.stride[1] + (c0 + c) * from.stride[2]]
-                                                      : from_f<T>(0.0f);
-    }
+  for (int i = threadIdx.x; i < kTile * kChannels; i += kThreads) {
+    const int t = i / kChannels, c = i % kChannels;
+    tile[i] = t0 + t < length && c0 + c < channels ? base[(t0 + t) * from.stride[1] + (c0 + c) * from.stride[2]]
+                                                    : from_f<T>(0.0f);
   }
 }
+
+// The tiles of one tensor's channels: a tensor map [B][L][C] where TMA reads it.
+struct Maps {
+  CUtensorMap map[4];
+};
 
 template <typename T> __device__ __forceinline__ float2 read_two(const T* tile, int token, int lane) {
   return Two<T>::open(reinterpret_cast<const typename Two<T>::word*>(tile + token * kChannels)[lane]);
 }
 
+// kVec: two channels at a time (they exist or not together)
 template <typename T, bool kVec>
-__device__ __forceinline__ void write_two(const m3_tensor& to, int64_t at, int c, int channels, float2 v) {
-  T* p = static_cast<T*>(to.data) + at;
+__device__ __forceinline__ void write_two(T* p, int64_t channel_stride, int c, int channels, float2 v) {
   if constexpr (kVec) {
-    if (c < channels) *reinterpret_cast<typename Two<T>::word*>(p + c) = Two<T>::close(v);
+    if (c < channels) *reinterpret_cast<typename Two<T>::word*>(p) = Two<T>::close(v);
   } else {
-    if (c < channels) p[c * to.stride[2]] = from_f<T>(v.x);
-    if (c + 1 < channels) p[(c + 1) * to.stride[2]] = from_f<T>(v.y);
+    if (c < channels) p[0] = from_f<T>(v.x);
+    if (c + 1 < channels) p[channel_stride] = from_f<T>(v.y);
   }
 }
 
-// Bits 0 .. kRun - 1: which tokens of this warp's run are resets. Read by the first lanes, a tile ahead.
-__device__ __forceinline__ bool read_reset(const m3_tensor& reset, int b, int64_t t, int64_t length, int lane) {
-  return reset.data && lane < kRun && t + lane < length &&
+template <typename T> __device__ __forceinline__ T* element(const m3_tensor& t, int b, int64_t token, int c) {
+  return static_cast<T*>(t.data) + b * t.stride[0] + token * t.stride[1] + c * t.stride[2];
+}
+
+// Whether token t + lane of this warp's run of `run` tokens is a reset. Read a tile ahead.
+__device__ __forceinline__ bool read_reset(const m3_tensor& reset, int b, int64_t t, int64_t length, int lane, int run) {
+  return reset.data && lane < run && t + lane < length &&
          static_cast<const uint8_t*>(reset.data)[b * reset.stride[0] + (t + lane) * reset.stride[1]] != 0;
 }
 
@@ -152,13 +167,12 @@ __device__ __forceinline__ void store_in(int rank, float4* local, float4 v) {
 constexpr int kMaxCluster = 16;
 
 // Shared memory of a CTA: kStages buffers of its tensors' tiles, the maps of its warps' runs (float4 = a, a', h0, h0'
-// of a lane's two channels; the backward's second array has the reverse maps' h0, h0'), and in clusters the maps of
-// the cluster's tiles, for even and odd groups of tiles.
-constexpr int kStages = 2;
+// of a lane's two channels; the backward has a second set for In), in clusters the maps of the cluster's tiles for
+// even and odd groups, the running state of 64 channels, and an mbarrier for each stage.
+constexpr int kStages = 2;  // a power of two
 template <typename T> __host__ __device__ constexpr int tile_bytes() { return kTile * kChannels * (int)sizeof(T); }
-constexpr int kRunMaps = kWarps * 32 * 16;
-__host__ __device__ constexpr int smem_bytes(int tile_bytes, int tensors, int run_maps, int cluster) {
-  return kStages * tensors * tile_bytes + run_maps * kRunMaps + (cluster > 1 ? 2 * cluster * 32 * 16 : 0);
+__host__ __device__ constexpr int smem_bytes(int tile_bytes, int tensors, int maps, int cluster) {
+  return kStages * tensors * tile_bytes + (maps + (cluster > 1 ? 2 * cluster : 0)) * 32 * 16 + 32 * 8 + kStages * 8;
 }
 
 // Leave `map`, of this CTA's tile, in every CTA of the cluster, and wait for theirs: maps[rank][lane].
@@ -178,267 +192,329 @@ __device__ __forceinline__ void join(float4& m, float4 next) {
   m.y = m.y == 0.0f || next.y == 0.0f ? 0.0f : fmaxf(m.y * next.y, kFloor);
 }
 
-// Forward. One pass over the inputs: a thread folds its run of 8 tokens into a map (a, h0), the maps of the 8 runs
+// What both kernels are made of: a CTA's channels and tiles, and the copies of the tiles into shared memory, kStages
+// deep. The tiles come in groups of `cluster`; step i is the i-th group that the kernel takes.
+template <typename T, int kTensors, int kThreads, bool kVec> struct Pipeline {
+  T* tiles;
+  uint32_t bars;  // shared-memory address of the stages' mbarriers
+  int64_t ntiles, groups;
+  int64_t newest = -1;  // the last step loaded
+  bool ok = true;
+
+  __device__ __forceinline__ void start(T* at, uint32_t bar) {
+    tiles = at;
+    bars = bar;
+    if constexpr (kVec) {
+      if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bars + 8 * s));
+        asm volatile("fence.mbarrier_init.release.cluster;");
+      }
+      __syncthreads();
+    }
+  }
+  __device__ __forceinline__ T* stage(int64_t i) { return tiles + (i & (kStages - 1)) * kTensors * kTile * kChannels; }
+  // Start on step i's tile t; everyone is done with the stage.
+  __device__ __forceinline__ void load(const Maps& maps, const m3_tensor* const* from, int64_t i, int64_t t, int b, int c0,
+                                       const m3_gated_args& a) {
+    if (t < 0 || t >= ntiles || !ok) return;
+    newest = i;
+    T* to = stage(i);
+    if constexpr (kVec) {
+      if (threadIdx.x == 0) {
+        const uint32_t bar = bars + 8 * (uint32_t)(i & (kStages - 1));
+        mbar_expect_tx(bar, kTensors * tile_bytes<T>());
+#pragma unroll
+        for (int k = 0; k < kTensors; ++k)
+          tma_load3(smem_u32(to + k * kTile * kChannels), &maps.map[k], c0, (int)(t * kTile), b, bar);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kTensors; ++k)
+        load_tile<T, kThreads>(to + k * kTile * kChannels, *from[k], b, t * kTile, c0, a.length, a.channels);
+    }
+  }
+  // Step i's tile is there; everyone is done with the step before. A wait that gave up (the error word says so) is not
+  // repeated: what is left runs through without it.
+  __device__ __forceinline__ const T* ready(int64_t i, int64_t t) {
+    if constexpr (kVec) {
+      if (ok && t < ntiles) ok = mbar_wait(bars + 8 * (uint32_t)(i & (kStages - 1)), (uint32_t)(i / kStages) & 1u);
+    }
+    __syncthreads();
+    return stage(i);
+  }
+  // After a wait that gave up: the copies still under way land before the block's shared memory goes.
+  __device__ __forceinline__ void finish() {
+    if constexpr (kVec) {
+      if (threadIdx.x == 0 && !ok)
+        for (int64_t i = newest - kStages + 1; i <= newest; ++i)
+          if (i >= 0) mbar_wait(bars + 8 * (uint32_t)(i & (kStages - 1)), (uint32_t)(i / kStages) & 1u);
+    }
+  }
+};
+
+// The first pass over a run: decays, inputs and the run's map. kWhole: every token is there and none is a reset.
+template <typename T, bool kWhole, int kRun>
+__device__ __forceinline__ float4 open_run(const T* forget, const T* value, int token, int lane, int n, uint32_t resets,
+                                           float2 (&keep)[kRun], float2 (&in)[kRun]) {
+  float4 m = make_float4(1.0f, 1.0f, 0.0f, 0.0f);
+  bool reset = false;
+#pragma unroll
+  for (int j = 0; j < kRun; ++j) {
+    if (!kWhole && j >= n) {
+      keep[j] = make_float2(1.0f, 1.0f);
+      in[j] = make_float2(0.0f, 0.0f);
+      continue;
+    }
+    const float2 f = read_two(forget, token + j, lane), v = read_two(value, token + j, lane);
+    float2 lose;
+    keep_lose(f.x, keep[j].x, lose.x);
+    keep_lose(f.y, keep[j].y, lose.y);
+    in[j] = make_float2(lose.x * v.x, lose.y * v.y);
+    if (!kWhole && (resets >> j & 1u)) {
+      m.z = m.w = 0.0f;
+      reset = true;
+    }
+    m.z = fmaf(keep[j].x, m.z, in[j].x);
+    m.w = fmaf(keep[j].y, m.w, in[j].y);
+    m.x *= keep[j].x;
+    m.y *= keep[j].y;
+  }
+  m.x = reset ? 0.0f : fmaxf(m.x, kFloor);
+  m.y = reset ? 0.0f : fmaxf(m.y, kFloor);
+  return m;
+}
+
+// Forward. One pass over the inputs: a thread folds its run of 16 tokens into a map (a, h0), the maps of the 4 runs
 // of a tile (and of a cluster's tiles) give every run the state before it, and the run is repeated from there
 // out of registers. CTAs walk a sequence's tiles one after another; where sequences and channels are too few to
 // fill the GPU, a cluster walks them together.
+constexpr int kFwdWarps = 4, kFwdThreads = 32 * kFwdWarps, kFwdRun = kTile / kFwdWarps;
+
 template <typename T, bool kGate, bool kVec>
-__global__ void __launch_bounds__(kThreads, 3) gated_fwd_kernel(const m3_gated_args a, int cluster) {
-  constexpr int kTensors = kGate ? 3 : 2, kElems = kTile * kChannels;
-  extern __shared__ __align__(16) uint8_t smem[];
-  T* tiles = reinterpret_cast<T*>(smem);
+__global__ void __launch_bounds__(kFwdThreads, 4)
+    gated_fwd_kernel(const __grid_constant__ Maps maps, const m3_gated_args a, const int cluster) {
+  constexpr int kTensors = kGate ? 3 : 2, kElems = kTile * kChannels, kRun = kFwdRun, kWarps = kFwdWarps;
+  extern __shared__ __align__(128) uint8_t smem[];
   float4* runs = reinterpret_cast<float4*>(smem + kStages * kTensors * tile_bytes<T>());
   float4* peers = runs + kWarps * 32;
+  float2* next = reinterpret_cast<float2*>(peers + (cluster > 1 ? 2 * cluster * 32 : 0));  // the state after the tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = cluster > 1 ? cluster_rank() : 0;
   const int b = blockIdx.y, c0 = blockIdx.x / cluster * kChannels, c = c0 + 2 * lane;
-  const int64_t ntiles = (a.length + kTile - 1) / kTile, groups = (ntiles + cluster - 1) / cluster;
-  auto load = [&](int64_t g) {
-    const int64_t t = g * cluster + rank;
-    if (g < groups && t < ntiles) {
-      T* to = tiles + (g % kStages) * kTensors * kElems;
-      load_tile<T, kVec>(to, a.forget, b, t * kTile, c0, a.length, a.channels);
-      load_tile<T, kVec>(to + kElems, a.value, b, t * kTile, c0, a.length, a.channels);
-      if constexpr (kGate) load_tile<T, kVec>(to + 2 * kElems, a.gate, b, t * kTile, c0, a.length, a.channels);
-    }
-    copies_commit();
-  };
+  Pipeline<T, kTensors, kFwdThreads, kVec> pipe;
+  pipe.ntiles = (a.length + kTile - 1) / kTile;
+  pipe.groups = (pipe.ntiles + cluster - 1) / cluster;
+  pipe.start(reinterpret_cast<T*>(smem), smem_u32(next + 32));
+  const m3_tensor* from[3] = {&a.forget, &a.value, &a.gate};
+  for (int i = 0; i < kStages - 1; ++i) pipe.load(maps, from, i, i * cluster + rank, b, c0, a);
   float2 carry = read_state(a.state, b, c, a.channels);  // the state before the group of tiles
-  for (int g = 0; g < kStages - 1; ++g) load(g);
-  bool flag = read_reset(a.reset, b, (int64_t)rank * kTile + warp * kRun, a.length, lane);
+  bool flag = read_reset(a.reset, b, (int64_t)rank * kTile + warp * kRun, a.length, lane, kRun);
+  T* to = element<T>(a.y, b, (int64_t)rank * kTile + warp * kRun, c);
   if (cluster > 1) {  // the others have started: their shared memory may be written
     cluster_arrive();
     cluster_wait();
   }
-  for (int64_t g = 0; g < groups; ++g) {
+  for (int64_t g = 0; g < pipe.groups; ++g, to += cluster * kTile * a.y.stride[1]) {
     const int64_t t = g * cluster + rank, t0 = t * kTile + warp * kRun;
     const uint32_t resets = __ballot_sync(0xffffffffu, flag);
-    flag = read_reset(a.reset, b, t0 + (int64_t)cluster * kTile, a.length, lane);
-    copies_wait<kStages - 2>();
-    __syncthreads();  // this group's tile is there, and everyone is done with the one before
-    load(g + kStages - 1);
-    const T* tile = tiles + (g % kStages) * kTensors * kElems;
+    flag = read_reset(a.reset, b, t0 + (int64_t)cluster * kTile, a.length, lane, kRun);
+    const T* tile = pipe.ready(g, t);
+    if (cluster == 1 && g > 0) carry = next[lane];
+    pipe.load(maps, from, g + kStages - 1, t + (kStages - 1) * cluster, b, c0, a);
     const int n = t0 >= a.length ? 0 : a.length - t0 < kRun ? (int)(a.length - t0) : kRun;  // tokens of this run
+    const bool whole = n == kRun && resets == 0;
     float2 keep[kRun], in[kRun];
-    float4 map = make_float4(1.0f, 1.0f, 0.0f, 0.0f);
-    float least = kFloor;
-#pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      keep[j] = make_float2(1.0f, 1.0f);
-      in[j] = make_float2(0.0f, 0.0f);
-      if (j < n) {
-        const float2 f = read_two(tile, warp * kRun + j, lane), v = read_two(tile + kElems, warp * kRun + j, lane);
-        float2 lose;
-        keep_lose(f.x, keep[j].x, lose.x);
-        keep_lose(f.y, keep[j].y, lose.y);
-        in[j] = make_float2(lose.x * v.x, lose.y * v.y);
-        if (resets >> j & 1u) map = make_float4(least = 0.0f, 0.0f, 0.0f, 0.0f);
-        map.z = fmaf(keep[j].x, map.z, in[j].x);
-        map.w = fmaf(keep[j].y, map.w, in[j].y);
-        map.x = fmaxf(map.x * keep[j].x, least);
-        map.y = fmaxf(map.y * keep[j].y, least);
-      }
-    }
+    const float4 map = whole ? open_run<T, true>(tile, tile + kElems, warp * kRun, lane, n, resets, keep, in)
+                             : open_run<T, false>(tile, tile + kElems, warp * kRun, lane, n, resets, keep, in);
     runs[warp * 32 + lane] = map;
     __syncthreads();
     float2 h = carry;  // the state before this CTA's tile
     if (cluster > 1) {
-      float4 whole = runs[lane];
+      float4 all = runs[lane];
       if (warp == 0)
-        for (int w = 1; w < kWarps; ++w) join(whole, runs[w * 32 + lane]);
-      float4* maps = peers + (g & 1) * cluster * 32;
-      exchange(maps, rank, cluster, warp, lane, whole);
+        for (int w = 1; w < kWarps; ++w) join(all, runs[w * 32 + lane]);
+      const float4* of = peers + (g & 1) * cluster * 32;
+      exchange(peers + (g & 1) * cluster * 32, rank, cluster, warp, lane, all);
       for (int r = 0; r < cluster; ++r) {
         if (r == rank) h = carry;
-        const float4 m = maps[r * 32 + lane];
-        carry.x = fold(m.x, m.z, carry.x);
-        carry.y = fold(m.y, m.w, carry.y);
+        carry = fold(of[r * 32 + lane], carry);
       }
     }
-    if (a.carry.data && warp == 0 && t < ntiles) {
-      float* to = static_cast<float*>(a.carry.data) + b * a.carry.stride[0] + t * a.carry.stride[1];
-      if (c < a.channels) to[c] = h.x;
-      if (c + 1 < a.channels) to[c + 1] = h.y;
+    if (a.carry.data && warp == 0 && t < pipe.ntiles) {
+      float* kept = static_cast<float*>(a.carry.data) + b * a.carry.stride[0] + t * a.carry.stride[1];
+      if (c < a.channels) kept[c] = h.x;
+      if (c + 1 < a.channels) kept[c + 1] = h.y;
     }
-    const int upto = cluster > 1 ? warp : kWarps;  // alone, the state after the tile is the next one's
-    float2 mine = h;
-    for (int w = 0; w < upto; ++w) {
-      if (w == warp) mine = h;
-      const float4 m = runs[w * 32 + lane];
-      h.x = fold(m.x, m.z, h.x);
-      h.y = fold(m.y, m.w, h.y);
-    }
-    if (cluster > 1) mine = h;
-    else carry = h;
-#pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      if (j >= n) break;
-      if (resets >> j & 1u) mine = make_float2(0.0f, 0.0f);
-      mine.x = fmaf(keep[j].x, mine.x, in[j].x);
-      mine.y = fmaf(keep[j].y, mine.y, in[j].y);
-      float2 y = mine;
+    for (int w = 0; w < warp; ++w) h = fold(runs[w * 32 + lane], h);
+    if (cluster == 1 && warp == kWarps - 1) next[lane] = fold(map, h);
+    auto finish = [&](int j) {
+      h.x = fmaf(keep[j].x, h.x, in[j].x);
+      h.y = fmaf(keep[j].y, h.y, in[j].y);
+      float2 y = h;
       if constexpr (kGate) {
         const float2 q = read_two(tile + 2 * kElems, warp * kRun + j, lane);
         y.x *= q.x * sigmoid_approx(q.x);
         y.y *= q.y * sigmoid_approx(q.y);
       }
-      write_two<T, kVec>(a.y, b * a.y.stride[0] + (t0 + j) * a.y.stride[1], c, a.channels, y);
+      write_two<T, kVec>(to + j * a.y.stride[1], a.y.stride[2], c, a.channels, y);
+    };
+    if (whole) {
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) finish(j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        if (j >= n) break;
+        if (resets >> j & 1u) h = make_float2(0.0f, 0.0f);
+        finish(j);
+      }
     }
+  }
+  pipe.finish();
+  if (cluster == 1) {
+    __syncthreads();
+    carry = next[lane];
   }
   if (rank == 0 && warp == 0) write_state(a.out_state, b, c, a.channels, carry);
 }
 
 // Backward, the tiles from the last to the first: the states of a tile come from the state kept before it, as in
-// the forward, and the gradients In run back through the same maps' a with h0 of their own.
+// the forward, and the gradients In run back through maps of the same a with h0 of their own.
+constexpr int kBwdWarps = 8, kBwdThreads = 32 * kBwdWarps, kBwdRun = kTile / kBwdWarps;
+
 template <typename T, bool kGate, bool kVec>
-__global__ void __launch_bounds__(kThreads, 2) gated_bwd_kernel(const m3_gated_args a, int cluster) {
-  constexpr int kTensors = kGate ? 4 : 3, kElems = kTile * kChannels;
-  extern __shared__ __align__(16) uint8_t smem[];
-  T* tiles = reinterpret_cast<T*>(smem);
+__global__ void __launch_bounds__(kBwdThreads, 2)
+    gated_bwd_kernel(const __grid_constant__ Maps maps, const m3_gated_args a, const int cluster) {
+  constexpr int kTensors = kGate ? 4 : 3, kElems = kTile * kChannels, kRun = kBwdRun, kWarps = kBwdWarps;
+  extern __shared__ __align__(128) uint8_t smem[];
   float4* runs = reinterpret_cast<float4*>(smem + kStages * kTensors * tile_bytes<T>());
   float4* back = runs + kWarps * 32;  // (a, a', In0, In0') of the runs from the back
   float4* peers = back + kWarps * 32;
+  float2* next = reinterpret_cast<float2*>(peers + (cluster > 1 ? 2 * cluster * 32 : 0));  // In before the tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = cluster > 1 ? cluster_rank() : 0;
   const int b = blockIdx.y, c0 = blockIdx.x / cluster * kChannels, c = c0 + 2 * lane;
-  const int64_t ntiles = (a.length + kTile - 1) / kTile, groups = (ntiles + cluster - 1) / cluster;
-  auto load = [&](int64_t g) {  // groups from the last, groups - 1, to 0
-    const int64_t t = g * cluster + rank;
-    if (g >= 0 && t < ntiles) {
-      T* to = tiles + (g % kStages) * kTensors * kElems;
-      load_tile<T, kVec>(to, a.forget, b, t * kTile, c0, a.length, a.channels);
-      load_tile<T, kVec>(to + kElems, a.value, b, t * kTile, c0, a.length, a.channels);
-      load_tile<T, kVec>(to + 2 * kElems, a.dy, b, t * kTile, c0, a.length, a.channels);
-      if constexpr (kGate) load_tile<T, kVec>(to + 3 * kElems, a.gate, b, t * kTile, c0, a.length, a.channels);
-    }
-    copies_commit();
-  };
+  Pipeline<T, kTensors, kBwdThreads, kVec> pipe;
+  pipe.ntiles = (a.length + kTile - 1) / kTile;
+  pipe.groups = (pipe.ntiles + cluster - 1) / cluster;
+  pipe.start(reinterpret_cast<T*>(smem), smem_u32(next + 32));
+  const m3_tensor* from[4] = {&a.forget, &a.value, &a.dy, &a.gate};
+  const int64_t last = (pipe.groups - 1) * cluster + rank;  // this CTA's tile of step 0; step i has last - i * cluster
+  // Only the first step's tile can be past the end. It is not loaded, so the stages' mbarriers do not count it: the
+  // pipeline's steps start at `skipped`.
+  const int skipped = last >= pipe.ntiles ? 1 : 0;
+  for (int i = 0; i < kStages - 1; ++i) pipe.load(maps, from, i - skipped, last - i * cluster, b, c0, a);
   auto before = [&](int64_t t) {  // the state kept before tile t
     float2 h = make_float2(0.0f, 0.0f);
-    if (t >= 0 && t < ntiles) {
-      const float* from = static_cast<const float*>(a.carry.data) + b * a.carry.stride[0] + t * a.carry.stride[1];
-      if (c < a.channels) h.x = from[c];
-      if (c + 1 < a.channels) h.y = from[c + 1];
+    if (t >= 0 && t < pipe.ntiles) {
+      const float* kept = static_cast<const float*>(a.carry.data) + b * a.carry.stride[0] + t * a.carry.stride[1];
+      if (c < a.channels) h.x = kept[c];
+      if (c + 1 < a.channels) h.y = kept[c + 1];
     }
     return h;
   };
   float2 carry = read_state(a.dstate, b, c, a.channels);  // In after the group of tiles
-  for (int i = 0; i < kStages - 1; ++i) load(groups - 1 - i);
-  bool flag = read_reset(a.reset, b, ((groups - 1) * cluster + rank) * kTile + warp * kRun, a.length, lane);
-  float2 kept = before((groups - 1) * cluster + rank);
+  bool flag = read_reset(a.reset, b, last * kTile + warp * kRun, a.length, lane, kRun);
+  float2 kept = before(last);
   if (cluster > 1) {
     cluster_arrive();
     cluster_wait();
   }
-  for (int64_t g = groups - 1; g >= 0; --g) {
-    const int64_t t = g * cluster + rank, t0 = t * kTile + warp * kRun;
+  for (int64_t i = 0; i < pipe.groups; ++i) {
+    const int64_t t = last - i * cluster, t0 = t * kTile + warp * kRun;
     const uint32_t resets = __ballot_sync(0xffffffffu, flag);
     float2 h = kept;
-    if (g > 0) {
-      flag = read_reset(a.reset, b, t0 - (int64_t)cluster * kTile, a.length, lane);
+    if (i + 1 < pipe.groups) {
+      flag = read_reset(a.reset, b, t0 - (int64_t)cluster * kTile, a.length, lane, kRun);
       kept = before(t - cluster);
     }
-    copies_wait<kStages - 2>();
-    __syncthreads();
-    load(g - (kStages - 1));
-    const T* tile = tiles + (g % kStages) * kTensors * kElems;
+    const T* tile = pipe.ready(i - skipped, t);
+    if (cluster == 1 && i > 0) carry = next[lane];
+    pipe.load(maps, from, i - skipped + kStages - 1, t - (kStages - 1) * cluster, b, c0, a);
     const int n = t0 >= a.length ? 0 : a.length - t0 < kRun ? (int)(a.length - t0) : kRun;
-    float2 keep[kRun], lose[kRun], dh[kRun];
-    float4 map = make_float4(1.0f, 1.0f, 0.0f, 0.0f);
-    float least = kFloor;
-#pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      keep[j] = make_float2(1.0f, 1.0f);
-      lose[j] = dh[j] = make_float2(0.0f, 0.0f);
-      if (j < n) {
-        const int token = warp * kRun + j;
-        const float2 f = read_two(tile, token, lane), v = read_two(tile + kElems, token, lane);
-        keep_lose(f.x, keep[j].x, lose[j].x);
-        keep_lose(f.y, keep[j].y, lose[j].y);
-        dh[j] = read_two(tile + 2 * kElems, token, lane);
-        if constexpr (kGate) {
-          const float2 q = read_two(tile + 3 * kElems, token, lane);
-          dh[j].x *= q.x * sigmoid_approx(q.x);
-          dh[j].y *= q.y * sigmoid_approx(q.y);
-        }
-        if (resets >> j & 1u) map = make_float4(least = 0.0f, 0.0f, 0.0f, 0.0f);
-        map.z = fmaf(keep[j].x, map.z, lose[j].x * v.x);
-        map.w = fmaf(keep[j].y, map.w, lose[j].y * v.y);
-        map.x = fmaxf(map.x * keep[j].x, least);
-        map.y = fmaxf(map.y * keep[j].y, least);
-      }
-    }
+    const bool whole = n == kRun && resets == 0;
+    float2 keep[kRun], in[kRun], dh[kRun];
+    const float4 map = whole ? open_run<T, true>(tile, tile + kElems, warp * kRun, lane, n, resets, keep, in)
+                             : open_run<T, false>(tile, tile + kElems, warp * kRun, lane, n, resets, keep, in);
     float4 rmap = make_float4(map.x, map.y, 0.0f, 0.0f);
 #pragma unroll
     for (int j = kRun - 1; j >= 0; --j) {
-      const bool cut = resets >> j & 1u;
-      rmap.z = cut ? 0.0f : keep[j].x * (dh[j].x + rmap.z);
-      rmap.w = cut ? 0.0f : keep[j].y * (dh[j].y + rmap.w);
+      dh[j] = make_float2(0.0f, 0.0f);
+      if (!whole && j >= n) continue;
+      dh[j] = read_two(tile + 2 * kElems, warp * kRun + j, lane);
+      if constexpr (kGate) {
+        const float2 q = read_two(tile + 3 * kElems, warp * kRun + j, lane);
+        dh[j].x *= q.x * sigmoid_approx(q.x);
+        dh[j].y *= q.y * sigmoid_approx(q.y);
+      }
+      rmap.z = keep[j].x * (dh[j].x + rmap.z);
+      rmap.w = keep[j].y * (dh[j].y + rmap.w);
+      if (!whole && (resets >> j & 1u)) rmap.z = rmap.w = 0.0f;
     }
     runs[warp * 32 + lane] = map;
     back[warp * 32 + lane] = rmap;
     __syncthreads();
-    float2 in = carry;  // In after this CTA's tile
+    float2 mine = carry;  // In after this CTA's tile, then after this run
     if (cluster > 1) {
-      float4 whole = back[(kWarps - 1) * 32 + lane];
+      float4 all = back[(kWarps - 1) * 32 + lane];
       if (warp == 0)
-        for (int w = kWarps - 2; w >= 0; --w) join(whole, back[w * 32 + lane]);
-      float4* maps = peers + (g & 1) * cluster * 32;
-      exchange(maps, rank, cluster, warp, lane, whole);
+        for (int w = kWarps - 2; w >= 0; --w) join(all, back[w * 32 + lane]);
+      const float4* of = peers + (i & 1) * cluster * 32;
+      exchange(peers + (i & 1) * cluster * 32, rank, cluster, warp, lane, all);
       for (int r = cluster - 1; r >= 0; --r) {
-        if (r == rank) in = carry;
-        const float4 m = maps[r * 32 + lane];
-        carry.x = fold(m.x, m.z, carry.x);
-        carry.y = fold(m.y, m.w, carry.y);
+        if (r == rank) mine = carry;
+        carry = fold(of[r * 32 + lane], carry);
       }
     }
-    for (int w = 0; w < warp; ++w) {
-      const float4 m = runs[w * 32 + lane];
-      h.x = fold(m.x, m.z, h.x);
-      h.y = fold(m.y, m.w, h.y);
-    }
-    const int downto = cluster > 1 ? warp + 1 : 0;
-    float2 mine = in;
-    for (int w = kWarps - 1; w >= downto; --w) {
-      if (w == warp) mine = in;
-      const float4 m = back[w * 32 + lane];
-      in.x = fold(m.x, m.z, in.x);
-      in.y = fold(m.y, m.w, in.y);
-    }
-    if (cluster > 1) mine = in;
-    else carry = in;
+    for (int w = 0; w < warp; ++w) h = fold(runs[w * 32 + lane], h);
+    for (int w = kWarps - 1; w > warp; --w) mine = fold(back[w * 32 + lane], mine);
+    if (cluster == 1 && warp == 0) next[lane] = fold(rmap, mine);
     float2 prev[kRun];  // h_{t-1} as token t sees it
 #pragma unroll
     for (int j = 0; j < kRun; ++j) {
-      if (resets >> j & 1u) h = make_float2(0.0f, 0.0f);
+      if (!whole && (resets >> j & 1u)) h = make_float2(0.0f, 0.0f);
       prev[j] = h;
-      const float2 v = j < n ? read_two(tile + kElems, warp * kRun + j, lane) : make_float2(0.0f, 0.0f);
-      h.x = fmaf(keep[j].x, h.x, lose[j].x * v.x);
-      h.y = fmaf(keep[j].y, h.y, lose[j].y * v.y);
+      h.x = fmaf(keep[j].x, h.x, in[j].x);
+      h.y = fmaf(keep[j].y, h.y, in[j].y);
     }
-#pragma unroll
-    for (int j = kRun - 1; j >= 0; --j) {
-      if (j >= n) continue;
+    auto finish = [&](int j) {
       const int token = warp * kRun + j;
-      const float2 v = read_two(tile + kElems, token, lane);
+      const float2 v = read_two(tile + kElems, token, lane), f = read_two(tile, token, lane);
       if constexpr (kGate) {
         const float2 q = read_two(tile + 3 * kElems, token, lane), dy = read_two(tile + 2 * kElems, token, lane);
         const float2 s = make_float2(sigmoid_approx(q.x), sigmoid_approx(q.y));
-        const float2 ht = make_float2(fmaf(keep[j].x, prev[j].x, lose[j].x * v.x), fmaf(keep[j].y, prev[j].y, lose[j].y * v.y));
-        write_two<T, kVec>(a.dgate, b * a.dgate.stride[0] + (t0 + j) * a.dgate.stride[1], c, a.channels,
+        const float2 ht = make_float2(fmaf(keep[j].x, prev[j].x, in[j].x), fmaf(keep[j].y, prev[j].y, in[j].y));
+        write_two<T, kVec>(element<T>(a.dgate, b, t0 + j, c), a.dgate.stride[2], c, a.channels,
                            make_float2(dy.x * ht.x * (s.x * fmaf(q.x, 1.0f - s.x, 1.0f)),
                                        dy.y * ht.y * (s.y * fmaf(q.y, 1.0f - s.y, 1.0f))));
       }
+      float2 again, lose;
+      keep_lose(f.x, again.x, lose.x);
+      keep_lose(f.y, again.y, lose.y);
       const float2 G = make_float2(dh[j].x + mine.x, dh[j].y + mine.y);
-      write_two<T, kVec>(a.dvalue, b * a.dvalue.stride[0] + (t0 + j) * a.dvalue.stride[1], c, a.channels,
-                         make_float2(G.x * lose[j].x, G.y * lose[j].y));
-      write_two<T, kVec>(a.dforget, b * a.dforget.stride[0] + (t0 + j) * a.dforget.stride[1], c, a.channels,
-                         make_float2(G.x * (prev[j].x - v.x) * (keep[j].x * lose[j].x),
-                                     G.y * (prev[j].y - v.y) * (keep[j].y * lose[j].y)));
-      const bool cut = resets >> j & 1u;
-      mine.x = cut ? 0.0f : keep[j].x * G.x;
-      mine.y = cut ? 0.0f : keep[j].y * G.y;
+      const float2 dv = make_float2(G.x * lose.x, G.y * lose.y);
+      write_two<T, kVec>(element<T>(a.dvalue, b, t0 + j, c), a.dvalue.stride[2], c, a.channels, dv);
+      write_two<T, kVec>(element<T>(a.dforget, b, t0 + j, c), a.dforget.stride[2], c, a.channels,
+                         make_float2(dv.x * keep[j].x * (prev[j].x - v.x), dv.y * keep[j].y * (prev[j].y - v.y)));
+      mine.x = keep[j].x * G.x;
+      mine.y = keep[j].y * G.y;
+    };
+    if (whole) {
+#pragma unroll
+      for (int j = kRun - 1; j >= 0; --j) finish(j);
+    } else {
+#pragma unroll
+      for (int j = kRun - 1; j >= 0; --j) {
+        if (j >= n) continue;
+        finish(j);
+        if (resets >> j & 1u) mine = make_float2(0.0f, 0.0f);
+      }
     }
+  }
+  pipe.finish();
+  if (cluster == 1) {
+    __syncthreads();
+    carry = next[lane];
   }
   if (a.dinitial.data && rank == 0 && warp == 0) write_state(a.dinitial, b, c, a.channels, carry);
 }
@@ -518,7 +594,36 @@ template <typename T> cudaError_t launch_step_token(const m3_gated_args& a, cuda
   return cudaGetLastError();
 }
 
-template <typename K> cudaError_t launch_tiles(K kernel, const m3_gated_args& a, int tile, int tensors, int run_maps, cudaStream_t stream) {
+// Whether TMA can read a tensor's tiles: unit stride along the channels, rows and start on 16 bytes.
+bool tma_reads(const m3_tensor& t, const m3_gated_args& a, int elem) {
+  auto whole = [&](int64_t stride, int64_t extent) { return extent == 1 || (stride > 0 && stride * elem % 16 == 0); };
+  return t.data == nullptr || (t.stride[2] == 1 && reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && whole(t.stride[0], a.batch) &&
+                               whole(t.stride[1], a.length) && a.length < INT32_MAX - kTile);
+}
+
+// Whether two neighbouring channels can be written as one word.
+bool pairs_written(const m3_tensor& t, const m3_gated_args& a, int elem) {
+  return t.data == nullptr || (a.channels % 2 == 0 && rows_aligned(t, elem, 2 * elem));
+}
+
+bool encode(CUtensorMap* map, const m3_tensor& t, const m3_gated_args& a, int elem) {
+  const PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+  if (enc == nullptr) return false;
+  const int64_t row = (int64_t)(a.channels * elem + 15) / 16 * 16;  // a stride that is never used
+  const int64_t token = a.length == 1 ? row : t.stride[1] * elem;
+  const cuuint64_t dims[3] = {(cuuint64_t)a.channels, (cuuint64_t)a.length, (cuuint64_t)a.batch};
+  const cuuint64_t strides[2] = {(cuuint64_t)token, (cuuint64_t)(a.batch == 1 ? row : t.stride[0] * elem)};
+  const cuuint32_t box[3] = {kChannels, kTile, 1}, step[3] = {1, 1, 1};
+  const CUtensorMapDataType type = t.dtype == M3_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : t.dtype == M3_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                       : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return enc(map, type, 3, t.data, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename K>
+cudaError_t launch_tiles(K kernel, const m3_gated_args& a, const Maps& maps, int threads, int tile, int tensors, int run_maps,
+                         cudaStream_t stream) {
   const int64_t ntiles = (a.length + kTile - 1) / kTile;
   const int64_t blocks = (int64_t)a.batch * ((a.channels + kChannels - 1) / kChannels);
   // CTAs that fit the GPU: a cluster takes a sequence's tiles together while its CTAs still have room at once
@@ -537,7 +642,7 @@ template <typename K> cudaError_t launch_tiles(K kernel, const m3_gated_args& a,
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((a.channels + kChannels - 1) / kChannels * cluster), (unsigned)a.batch);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -546,33 +651,39 @@ template <typename K> cudaError_t launch_tiles(K kernel, const m3_gated_args& a,
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, a, cluster);
+  return cudaLaunchKernelEx(&cfg, kernel, maps, a, cluster);
 }
 
 template <typename T> cudaError_t launch_fwd(const m3_gated_args& a, cudaStream_t stream) {
   if (a.length == 1) return launch_step_token<T>(a, stream);
-  constexpr int kElem = sizeof(T), kWord = 16 / kElem;
-  const bool vec = a.channels % kWord == 0 && rows_aligned(a.value, kElem, 16) && rows_aligned(a.forget, kElem, 16) &&
-                   rows_aligned(a.gate, kElem, 16) && rows_aligned(a.y, kElem, 2 * kElem);
-  constexpr int tile = tile_bytes<T>();
+  constexpr int kElem = sizeof(T), tile = tile_bytes<T>();
+  Maps maps = {};
+  const bool vec = tma_reads(a.forget, a, kElem) && tma_reads(a.value, a, kElem) && tma_reads(a.gate, a, kElem) &&
+                   pairs_written(a.y, a, kElem);
+  if (vec && !(encode(&maps.map[0], a.forget, a, kElem) && encode(&maps.map[1], a.value, a, kElem) &&
+               (a.gate.data == nullptr || encode(&maps.map[2], a.gate, a, kElem))))
+    return cudaErrorInvalidValue;
   if (a.gate.data)
-    return vec ? launch_tiles(gated_fwd_kernel<T, true, true>, a, tile, 3, 1, stream)
-               : launch_tiles(gated_fwd_kernel<T, true, false>, a, tile, 3, 1, stream);
-  return vec ? launch_tiles(gated_fwd_kernel<T, false, true>, a, tile, 2, 1, stream)
-             : launch_tiles(gated_fwd_kernel<T, false, false>, a, tile, 2, 1, stream);
+    return launch_tiles(vec ? gated_fwd_kernel<T, true, true> : gated_fwd_kernel<T, true, false>, a, maps, kFwdThreads, tile, 3,
+                        kFwdWarps, stream);
+  return launch_tiles(vec ? gated_fwd_kernel<T, false, true> : gated_fwd_kernel<T, false, false>, a, maps, kFwdThreads, tile, 2,
+                      kFwdWarps, stream);
 }
 
 template <typename T> cudaError_t launch_bwd(const m3_gated_args& a, cudaStream_t stream) {
-  constexpr int kElem = sizeof(T), kWord = 16 / kElem;
-  const bool vec = a.channels % kWord == 0 && rows_aligned(a.value, kElem, 16) && rows_aligned(a.forget, kElem, 16) &&
-                   rows_aligned(a.gate, kElem, 16) && rows_aligned(a.dy, kElem, 16) && rows_aligned(a.dvalue, kElem, 2 * kElem) &&
-                   rows_aligned(a.dforget, kElem, 2 * kElem) && rows_aligned(a.dgate, kElem, 2 * kElem);
-  constexpr int tile = tile_bytes<T>();
+  constexpr int kElem = sizeof(T), tile = tile_bytes<T>();
+  Maps maps = {};
+  const bool vec = tma_reads(a.forget, a, kElem) && tma_reads(a.value, a, kElem) && tma_reads(a.dy, a, kElem) &&
+                   tma_reads(a.gate, a, kElem) && pairs_written(a.dvalue, a, kElem) && pairs_written(a.dforget, a, kElem) &&
+                   pairs_written(a.dgate, a, kElem);
+  if (vec && !(encode(&maps.map[0], a.forget, a, kElem) && encode(&maps.map[1], a.value, a, kElem) &&
+               encode(&maps.map[2], a.dy, a, kElem) && (a.gate.data == nullptr || encode(&maps.map[3], a.gate, a, kElem))))
+    return cudaErrorInvalidValue;
   if (a.gate.data)
-    return vec ? launch_tiles(gated_bwd_kernel<T, true, true>, a, tile, 4, 2, stream)
-               : launch_tiles(gated_bwd_kernel<T, true, false>, a, tile, 4, 2, stream);
-  return vec ? launch_tiles(gated_bwd_kernel<T, false, true>, a, tile, 3, 2, stream)
-             : launch_tiles(gated_bwd_kernel<T, false, false>, a, tile, 3, 2, stream);
+    return launch_tiles(vec ? gated_bwd_kernel<T, true, true> : gated_bwd_kernel<T, true, false>, a, maps, kBwdThreads, tile, 4,
+                        2 * kBwdWarps, stream);
+  return launch_tiles(vec ? gated_bwd_kernel<T, false, true> : gated_bwd_kernel<T, false, false>, a, maps, kBwdThreads, tile, 3,
+                      2 * kBwdWarps, stream);
 }
 
 bool shaped(const m3_tensor& t, int ndim, int dtype) { return t.data == nullptr || (t.ndim == ndim && t.dtype == dtype); }
