@@ -111,20 +111,34 @@ template <typename T> __device__ __forceinline__ float2 read_two(const T* tile, 
   return Two<T>::open(reinterpret_cast<const typename Two<T>::word*>(tile + token * kChannels)[lane]);
 }
 
-// kVec: two channels at a time (they exist or not together)
-template <typename T, bool kVec>
-__device__ __forceinline__ void write_two(T* p, int64_t channel_stride, int c, int channels, float2 v) {
-  if constexpr (kVec) {
-    if (c < channels) *reinterpret_cast<typename Two<T>::word*>(p) = Two<T>::close(v);
-  } else {
-    if (c < channels) p[0] = from_f<T>(v.x);
-    if (c + 1 < channels) p[channel_stride] = from_f<T>(v.y);
-  }
-}
+// Where a thread's two channels of its run's tokens go in an output: `at` is the CTA's tile, the same for all threads,
+// and the rest an offset in 32 bits (kVec: 64 token strides fit them).
+template <typename T, bool kVec> struct Rows {
+  T* at;
+  int64_t stride, channel_stride;
+  uint32_t first;
+  int c, channels;
 
-template <typename T> __device__ __forceinline__ T* element(const m3_tensor& t, int b, int64_t token, int c) {
-  return static_cast<T*>(t.data) + b * t.stride[0] + token * t.stride[1] + c * t.stride[2];
-}
+  __device__ __forceinline__ void start(const m3_tensor& t, int b, int64_t token, int c0, int run0, int lane, int channels_) {
+    at = static_cast<T*>(t.data) + b * t.stride[0] + token * t.stride[1] + c0 * t.stride[2];
+    stride = t.stride[1];
+    channel_stride = t.stride[2];
+    c = c0 + 2 * lane;
+    channels = channels_;
+    first = kVec ? (uint32_t)run0 * (uint32_t)stride + 2 * lane : 0;
+    if (!kVec) at += run0 * stride + 2 * lane * channel_stride;
+  }
+  __device__ __forceinline__ void go(int64_t tokens) { at += tokens * stride; }
+  __device__ __forceinline__ void write(int j, float2 v) const {
+    if constexpr (kVec) {  // both channels exist, or neither
+      if (c < channels) *reinterpret_cast<typename Two<T>::word*>(at + (first + (uint32_t)j * (uint32_t)stride)) = Two<T>::close(v);
+    } else {
+      T* p = at + j * stride;
+      if (c < channels) p[0] = from_f<T>(v.x);
+      if (c + 1 < channels) p[channel_stride] = from_f<T>(v.y);
+    }
+  }
+};
 
 // Whether token t + lane of this warp's run of `run` tokens is a reset. Read a tile ahead.
 __device__ __forceinline__ bool read_reset(const m3_tensor& reset, int b, int64_t t, int64_t length, int lane, int run) {
@@ -156,33 +170,64 @@ __device__ __forceinline__ int cluster_rank() {
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ void store_in(int rank, float4* local, float4 v) {
-  uint32_t at;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
-               : "=r"(at)
-               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(local))), "r"(rank));
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+// Send 16 bytes to the same place in the shared memory of CTA `rank`, counted there by the mbarrier at `bar`. No
+// fence is involved: a cluster barrier's release would wait for every store to global memory before it.
+__device__ __forceinline__ void send(int rank, uint32_t to, uint32_t bar, float4 v) {
+  uint32_t there, counted;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(to), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(counted) : "r"(bar), "r"(rank));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(there),
+               "r"(__float_as_uint(v.x)), "r"(__float_as_uint(v.y)), "r"(__float_as_uint(v.z)), "r"(__float_as_uint(v.w)),
+               "r"(counted)
+               : "memory");
 }
 
 constexpr int kMaxCluster = 16;
 
 // Shared memory of a CTA: kStages buffers of its tensors' tiles, the maps of its warps' runs (float4 = a, a', h0, h0'
 // of a lane's two channels; the backward has a second set for In), in clusters the maps of the cluster's tiles for
-// even and odd groups, the running state of 64 channels, and an mbarrier for each stage.
+// even and odd groups, the running state of 64 channels, an mbarrier for each stage and two for the exchange.
 constexpr int kStages = 2;  // a power of two
 template <typename T> __host__ __device__ constexpr int tile_bytes() { return kTile * kChannels * (int)sizeof(T); }
 __host__ __device__ constexpr int smem_bytes(int tile_bytes, int tensors, int maps, int cluster) {
-  return kStages * tensors * tile_bytes + (maps + (cluster > 1 ? 2 * cluster : 0)) * 32 * 16 + 32 * 8 + kStages * 8;
+  return kStages * tensors * tile_bytes + (maps + (cluster > 1 ? 2 * cluster : 0)) * 32 * 16 + 32 * 8 + (kStages + 2) * 8;
 }
 
-// Leave `map`, of this CTA's tile, in every CTA of the cluster, and wait for theirs: maps[rank][lane].
-__device__ __forceinline__ void exchange(float4* maps, int rank, int cluster, int warp, int lane, float4 map) {
-  if (warp == 0)
-    for (int r = 0; r < cluster; ++r) store_in(r, maps + rank * 32 + lane, map);
-  __syncwarp();
-  cluster_arrive();
-  cluster_wait();
-}
+// The exchange of a cluster: step i, every CTA leaves its tile's map in every CTA, maps[rank][lane], for even and odd
+// steps apart. A CTA sends in step i + 2, over step i's maps, only when it has everyone's of step i + 1, and those
+// were sent after their senders had read step i's.
+struct Exchange {
+  float4* maps;
+  uint32_t bars;
+  int rank, cluster;
+
+  __device__ __forceinline__ void start() {
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < 2; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bars + 8 * s));
+      asm volatile("fence.mbarrier_init.release.cluster;");
+    }
+    __syncthreads();
+    cluster_arrive();  // the others have started, and their barriers are there
+    cluster_wait();
+  }
+  // `all`: warp 0's lanes have the tile's map. Returns the step's maps.
+  __device__ __forceinline__ const float4* run(int64_t i, int warp, int lane, float4 all, bool& ok) {
+    float4* at = maps + (i & 1) * cluster * 32;
+    const uint32_t bar = bars + 8 * (uint32_t)(i & 1);
+    if (threadIdx.x == 0) mbar_expect_tx(bar, (uint32_t)cluster * 32 * 16);
+    if (warp == 0)
+      for (int r = 0; r < cluster; ++r) send(r, smem_u32(at + rank * 32 + lane), bar, all);
+    if (ok) ok = mbar_wait(bar, (uint32_t)(i >> 1) & 1u);
+    __syncwarp();
+    return at;
+  }
+  // No CTA leaves while another could still send to it (after a wait that gave up).
+  __device__ __forceinline__ void finish() {
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+  }
+};
 
 // The map of one run after another.
 __device__ __forceinline__ void join(float4& m, float4 next) {
@@ -252,30 +297,32 @@ template <typename T, int kTensors, int kThreads, bool kVec> struct Pipeline {
   }
 };
 
-// The first pass over a run: decays, inputs and the run's map. kWhole: every token is there and none is a reset.
-template <typename T, bool kWhole, int kRun>
+// The first pass over a run: decays f, inputs (1 - f) value (kLose: 1 - f alone) and the run's map. kWhole: every
+// token is there and none is a reset.
+template <typename T, bool kWhole, bool kLose, int kRun>
 __device__ __forceinline__ float4 open_run(const T* forget, const T* value, int token, int lane, int n, uint32_t resets,
-                                           float2 (&keep)[kRun], float2 (&in)[kRun]) {
+                                           float2 (&keep)[kRun], float2 (&other)[kRun]) {
   float4 m = make_float4(1.0f, 1.0f, 0.0f, 0.0f);
   bool reset = false;
 #pragma unroll
   for (int j = 0; j < kRun; ++j) {
     if (!kWhole && j >= n) {
       keep[j] = make_float2(1.0f, 1.0f);
-      in[j] = make_float2(0.0f, 0.0f);
+      other[j] = make_float2(0.0f, 0.0f);
       continue;
     }
     const float2 f = read_two(forget, token + j, lane), v = read_two(value, token + j, lane);
     float2 lose;
     keep_lose(f.x, keep[j].x, lose.x);
     keep_lose(f.y, keep[j].y, lose.y);
-    in[j] = make_float2(lose.x * v.x, lose.y * v.y);
+    const float2 in = make_float2(lose.x * v.x, lose.y * v.y);
+    other[j] = kLose ? lose : in;
     if (!kWhole && (resets >> j & 1u)) {
       m.z = m.w = 0.0f;
       reset = true;
     }
-    m.z = fmaf(keep[j].x, m.z, in[j].x);
-    m.w = fmaf(keep[j].y, m.w, in[j].y);
+    m.z = fmaf(keep[j].x, m.z, in.x);
+    m.w = fmaf(keep[j].y, m.w, in.y);
     m.x *= keep[j].x;
     m.y *= keep[j].y;
   }
@@ -309,12 +356,11 @@ __global__ void __launch_bounds__(kFwdThreads, 4)
   for (int i = 0; i < kStages - 1; ++i) pipe.load(maps, from, i, i * cluster + rank, b, c0, a);
   float2 carry = read_state(a.state, b, c, a.channels);  // the state before the group of tiles
   bool flag = read_reset(a.reset, b, (int64_t)rank * kTile + warp * kRun, a.length, lane, kRun);
-  T* to = element<T>(a.y, b, (int64_t)rank * kTile + warp * kRun, c);
-  if (cluster > 1) {  // the others have started: their shared memory may be written
-    cluster_arrive();
-    cluster_wait();
-  }
-  for (int64_t g = 0; g < pipe.groups; ++g, to += cluster * kTile * a.y.stride[1]) {
+  Rows<T, kVec> y;
+  y.start(a.y, b, (int64_t)rank * kTile, c0, warp * kRun, lane, a.channels);
+  Exchange exchange{peers, smem_u32(next + 32) + 8 * kStages, rank, cluster};
+  if (cluster > 1) exchange.start();
+  for (int64_t g = 0; g < pipe.groups; ++g, y.go(cluster * kTile)) {
     const int64_t t = g * cluster + rank, t0 = t * kTile + warp * kRun;
     const uint32_t resets = __ballot_sync(0xffffffffu, flag);
     flag = read_reset(a.reset, b, t0 + (int64_t)cluster * kTile, a.length, lane, kRun);
@@ -324,8 +370,8 @@ __global__ void __launch_bounds__(kFwdThreads, 4)
     const int n = t0 >= a.length ? 0 : a.length - t0 < kRun ? (int)(a.length - t0) : kRun;  // tokens of this run
     const bool whole = n == kRun && resets == 0;
     float2 keep[kRun], in[kRun];
-    const float4 map = whole ? open_run<T, true>(tile, tile + kElems, warp * kRun, lane, n, resets, keep, in)
-                             : open_run<T, false>(tile, tile + kElems, warp * kRun, lane, n, resets, keep, in);
+    const float4 map = whole ? open_run<T, true, false>(tile, tile + kElems, warp * kRun, lane, n, resets, keep, in)
+                             : open_run<T, false, false>(tile, tile + kElems, warp * kRun, lane, n, resets, keep, in);
     runs[warp * 32 + lane] = map;
     __syncthreads();
     float2 h = carry;  // the state before this CTA's tile
@@ -333,8 +379,7 @@ __global__ void __launch_bounds__(kFwdThreads, 4)
       float4 all = runs[lane];
       if (warp == 0)
         for (int w = 1; w < kWarps; ++w) join(all, runs[w * 32 + lane]);
-      const float4* of = peers + (g & 1) * cluster * 32;
-      exchange(peers + (g & 1) * cluster * 32, rank, cluster, warp, lane, all);
+      const float4* of = exchange.run(g, warp, lane, all, pipe.ok);
       for (int r = 0; r < cluster; ++r) {
         if (r == rank) h = carry;
         carry = fold(of[r * 32 + lane], carry);
@@ -350,13 +395,13 @@ __global__ void __launch_bounds__(kFwdThreads, 4)
     auto finish = [&](int j) {
       h.x = fmaf(keep[j].x, h.x, in[j].x);
       h.y = fmaf(keep[j].y, h.y, in[j].y);
-      float2 y = h;
+      float2 out = h;
       if constexpr (kGate) {
         const float2 q = read_two(tile + 2 * kElems, warp * kRun + j, lane);
-        y.x *= q.x * sigmoid_approx(q.x);
-        y.y *= q.y * sigmoid_approx(q.y);
+        out.x *= q.x * sigmoid_approx(q.x);
+        out.y *= q.y * sigmoid_approx(q.y);
       }
-      write_two<T, kVec>(to + j * a.y.stride[1], a.y.stride[2], c, a.channels, y);
+      y.write(j, out);
     };
     if (whole) {
 #pragma unroll
@@ -371,7 +416,8 @@ __global__ void __launch_bounds__(kFwdThreads, 4)
     }
   }
   pipe.finish();
-  if (cluster == 1) {
+  if (cluster > 1) exchange.finish();
+  else {
     __syncthreads();
     carry = next[lane];
   }
@@ -416,10 +462,12 @@ __global__ void __launch_bounds__(kBwdThreads, 2)
   float2 carry = read_state(a.dstate, b, c, a.channels);  // In after the group of tiles
   bool flag = read_reset(a.reset, b, last * kTile + warp * kRun, a.length, lane, kRun);
   float2 kept = before(last);
-  if (cluster > 1) {
-    cluster_arrive();
-    cluster_wait();
-  }
+  Rows<T, kVec> dvalue, dforget, dgate;
+  dvalue.start(a.dvalue, b, last * kTile, c0, warp * kRun, lane, a.channels);
+  dforget.start(a.dforget, b, last * kTile, c0, warp * kRun, lane, a.channels);
+  if constexpr (kGate) dgate.start(a.dgate, b, last * kTile, c0, warp * kRun, lane, a.channels);
+  Exchange exchange{peers, smem_u32(next + 32) + 8 * kStages, rank, cluster};
+  if (cluster > 1) exchange.start();
   for (int64_t i = 0; i < pipe.groups; ++i) {
     const int64_t t = last - i * cluster, t0 = t * kTile + warp * kRun;
     const uint32_t resets = __ballot_sync(0xffffffffu, flag);
@@ -433,19 +481,20 @@ __global__ void __launch_bounds__(kBwdThreads, 2)
     pipe.load(maps, from, i - skipped + kStages - 1, t - (kStages - 1) * cluster, b, c0, a);
     const int n = t0 >= a.length ? 0 : a.length - t0 < kRun ? (int)(a.length - t0) : kRun;
     const bool whole = n == kRun && resets == 0;
-    float2 keep[kRun], in[kRun], dh[kRun];
-    const float4 map = whole ? open_run<T, true>(tile, tile + kElems, warp * kRun, lane, n, resets, keep, in)
-                             : open_run<T, false>(tile, tile + kElems, warp * kRun, lane, n, resets, keep, in);
+    float2 keep[kRun], lose[kRun], dh[kRun], slope[kRun];  // slope: sigmoid(gate)
+    const float4 map = whole ? open_run<T, true, true>(tile, tile + kElems, warp * kRun, lane, n, resets, keep, lose)
+                             : open_run<T, false, true>(tile, tile + kElems, warp * kRun, lane, n, resets, keep, lose);
     float4 rmap = make_float4(map.x, map.y, 0.0f, 0.0f);
 #pragma unroll
     for (int j = kRun - 1; j >= 0; --j) {
-      dh[j] = make_float2(0.0f, 0.0f);
+      dh[j] = slope[j] = make_float2(0.0f, 0.0f);
       if (!whole && j >= n) continue;
       dh[j] = read_two(tile + 2 * kElems, warp * kRun + j, lane);
       if constexpr (kGate) {
         const float2 q = read_two(tile + 3 * kElems, warp * kRun + j, lane);
-        dh[j].x *= q.x * sigmoid_approx(q.x);
-        dh[j].y *= q.y * sigmoid_approx(q.y);
+        slope[j] = make_float2(sigmoid_approx(q.x), sigmoid_approx(q.y));
+        dh[j].x *= q.x * slope[j].x;
+        dh[j].y *= q.y * slope[j].y;
       }
       rmap.z = keep[j].x * (dh[j].x + rmap.z);
       rmap.w = keep[j].y * (dh[j].y + rmap.w);
@@ -459,8 +508,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2)
       float4 all = back[(kWarps - 1) * 32 + lane];
       if (warp == 0)
         for (int w = kWarps - 2; w >= 0; --w) join(all, back[w * 32 + lane]);
-      const float4* of = peers + (i & 1) * cluster * 32;
-      exchange(peers + (i & 1) * cluster * 32, rank, cluster, warp, lane, all);
+      const float4* of = exchange.run(i, warp, lane, all, pipe.ok);
       for (int r = cluster - 1; r >= 0; --r) {
         if (r == rank) mine = carry;
         carry = fold(of[r * 32 + lane], carry);
@@ -472,32 +520,29 @@ __global__ void __launch_bounds__(kBwdThreads, 2)
     float2 prev[kRun];  // h_{t-1} as token t sees it
 #pragma unroll
     for (int j = 0; j < kRun; ++j) {
+      if (!whole && j >= n) break;
       if (!whole && (resets >> j & 1u)) h = make_float2(0.0f, 0.0f);
       prev[j] = h;
-      h.x = fmaf(keep[j].x, h.x, in[j].x);
-      h.y = fmaf(keep[j].y, h.y, in[j].y);
+      const float2 v = read_two(tile + kElems, warp * kRun + j, lane);
+      h.x = fmaf(keep[j].x, h.x, lose[j].x * v.x);
+      h.y = fmaf(keep[j].y, h.y, lose[j].y * v.y);
     }
     auto finish = [&](int j) {
       const int token = warp * kRun + j;
-      const float2 v = read_two(tile + kElems, token, lane), f = read_two(tile, token, lane);
-      if constexpr (kGate) {
+      const float2 v = read_two(tile + kElems, token, lane);
+      if constexpr (kGate) {  // dy h (s + gate s (1 - s))
         const float2 q = read_two(tile + 3 * kElems, token, lane), dy = read_two(tile + 2 * kElems, token, lane);
-        const float2 s = make_float2(sigmoid_approx(q.x), sigmoid_approx(q.y));
-        const float2 ht = make_float2(fmaf(keep[j].x, prev[j].x, in[j].x), fmaf(keep[j].y, prev[j].y, in[j].y));
-        write_two<T, kVec>(element<T>(a.dgate, b, t0 + j, c), a.dgate.stride[2], c, a.channels,
-                           make_float2(dy.x * ht.x * (s.x * fmaf(q.x, 1.0f - s.x, 1.0f)),
-                                       dy.y * ht.y * (s.y * fmaf(q.y, 1.0f - s.y, 1.0f))));
+        const float2 s = slope[j];
+        const float2 ht = make_float2(fmaf(keep[j].x, prev[j].x, lose[j].x * v.x), fmaf(keep[j].y, prev[j].y, lose[j].y * v.y));
+        const float2 qs = make_float2(q.x * s.x, q.y * s.y);
+        dgate.write(j, make_float2(dy.x * ht.x * fmaf(qs.x, 1.0f - s.x, s.x), dy.y * ht.y * fmaf(qs.y, 1.0f - s.y, s.y)));
       }
-      float2 again, lose;
-      keep_lose(f.x, again.x, lose.x);
-      keep_lose(f.y, again.y, lose.y);
       const float2 G = make_float2(dh[j].x + mine.x, dh[j].y + mine.y);
-      const float2 dv = make_float2(G.x * lose.x, G.y * lose.y);
-      write_two<T, kVec>(element<T>(a.dvalue, b, t0 + j, c), a.dvalue.stride[2], c, a.channels, dv);
-      write_two<T, kVec>(element<T>(a.dforget, b, t0 + j, c), a.dforget.stride[2], c, a.channels,
-                         make_float2(dv.x * keep[j].x * (prev[j].x - v.x), dv.y * keep[j].y * (prev[j].y - v.y)));
+      const float2 dv = make_float2(G.x * lose[j].x, G.y * lose[j].y);
       mine.x = keep[j].x * G.x;
       mine.y = keep[j].y * G.y;
+      dvalue.write(j, dv);
+      dforget.write(j, make_float2(mine.x * lose[j].x * (prev[j].x - v.x), mine.y * lose[j].y * (prev[j].y - v.y)));
     };
     if (whole) {
 #pragma unroll
@@ -510,9 +555,13 @@ __global__ void __launch_bounds__(kBwdThreads, 2)
         if (resets >> j & 1u) mine = make_float2(0.0f, 0.0f);
       }
     }
+    dvalue.go(-cluster * kTile);
+    dforget.go(-cluster * kTile);
+    if constexpr (kGate) dgate.go(-cluster * kTile);
   }
   pipe.finish();
-  if (cluster == 1) {
+  if (cluster > 1) exchange.finish();
+  else {
     __syncthreads();
     carry = next[lane];
   }
@@ -601,9 +650,9 @@ bool tma_reads(const m3_tensor& t, const m3_gated_args& a, int elem) {
                                whole(t.stride[1], a.length) && a.length < INT32_MAX - kTile);
 }
 
-// Whether two neighbouring channels can be written as one word.
+// Whether two neighbouring channels can be written as one word, a tile of 64 tokens within offsets of 32 bits.
 bool pairs_written(const m3_tensor& t, const m3_gated_args& a, int elem) {
-  return t.data == nullptr || (a.channels % 2 == 0 && rows_aligned(t, elem, 2 * elem));
+  return t.data == nullptr || (a.channels % 2 == 0 && rows_aligned(t, elem, 2 * elem) && t.stride[1] >= 0 && t.stride[1] < (1 << 23));
 }
 
 bool encode(CUtensorMap* map, const m3_tensor& t, const m3_gated_args& a, int elem) {
