@@ -504,6 +504,7 @@ def gemv(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
 _TENSOR_CODES = {torch.float32: M3_F32, torch.float16: M3_F16, torch.bfloat16: M3_BF16, torch.uint8: M3_U8,
                  torch.bool: M3_U8}
 _ABSENT = (0,) * 8
+_NO_TRAINING = _ABSENT * 7  # carry, dy, dstate and the gradients
 _PAD = {1: (0,) * 5, 2: (0,) * 4, 3: (0,) * 3}
 
 _GATED_FORMAT = struct.Struct("=qiiii" + "8q" * 14)
@@ -518,8 +519,21 @@ def _words(t: torch.Tensor | None) -> tuple:
     return (t.data_ptr(), _TENSOR_CODES[t.dtype] | n << 32, *t.stride(), *_PAD[n])
 
 
+def _token_words(t: torch.Tensor | None) -> tuple:
+    """``[B, C]`` as the one token of a ``[B, 1, C]`` tensor."""
+    if t is None:
+        return _ABSENT
+    batch, channel = t.stride()
+    return (t.data_ptr(), _TENSOR_CODES[t.dtype] | 3 << 32, batch, 0, channel, 0, 0, 0)
+
+
+# The raw handle of a device's current stream; torch.cuda.current_stream builds an object around it, which costs
+# as much as a kernel launch.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device.index)
 
 
 @torch.compiler.disable
@@ -530,7 +544,20 @@ def gated_scan_forward(value, forget, gate, reset, state, *, y, out_state, carry
     batch, length, channels = value.shape
     args = _GATED_FORMAT.pack(length, batch, channels, value.device.index, 0, *_words(value), *_words(forget),
                               *_words(gate), *_words(reset), *_words(state), *_words(y), *_words(out_state),
-                              *_words(carry), *_ABSENT, *_ABSENT, *_ABSENT, *_ABSENT, *_ABSENT, *_ABSENT)
+                              *_words(carry), *_NO_TRAINING[8:])
+    rc = lib.m3_gated_scan_fwd(args, _stream(value.device))
+    if rc:
+        _check(rc, lib)
+
+
+@torch.compiler.disable
+def gated_step(value, forget, gate, state, *, y, out_state) -> None:
+    """``m3_gated_scan_fwd`` of one token: ``[B, C]`` tensors."""
+    lib = load()
+    batch, channels = value.shape
+    args = _GATED_FORMAT.pack(1, batch, channels, value.device.index, 0, *_token_words(value), *_token_words(forget),
+                              *_token_words(gate), *_ABSENT, *_words(state), *_token_words(y), *_words(out_state),
+                              *_NO_TRAINING)
     rc = lib.m3_gated_scan_fwd(args, _stream(value.device))
     if rc:
         _check(rc, lib)

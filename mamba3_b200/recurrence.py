@@ -16,7 +16,6 @@ import math
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 from torch.nn import functional as F
 
 from . import _ext
@@ -83,8 +82,9 @@ class _GatedScan(torch.autograd.Function):
         return y, out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dstate):
+        if torch.is_grad_enabled():  # create_graph=True
+            raise RuntimeError("gated_scan is differentiable once: its gradient has no gradient on CUDA")
         value, forget, gate, reset, carry = ctx.saved_tensors
         dy = torch.zeros(value.shape, device=value.device, dtype=value.dtype) if dy is None else dy
         dvalue, dforget, dgate, dinitial = _ext.gated_scan_backward(value, forget, gate, reset, carry, dy, dstate,
@@ -131,22 +131,33 @@ def gated_step(value: torch.Tensor, forget: torch.Tensor, state: torch.Tensor, g
         raise ValueError("value must have shape [B, C]")
     if state is None:
         raise ValueError("gated_step needs a state; start from zeros")
-    value, forget = value.unsqueeze(1), forget.unsqueeze(1) if forget.dim() == 2 else forget
-    gate = gate.unsqueeze(1) if gate is not None and gate.dim() == 2 else gate
-    _validate(value, forget, gate, state, None)
-    if out_state is not None and (out_state.shape != state.shape or out_state.dtype != torch.float32
-                                  or out_state.device != state.device):
+    shape, dtype, device = value.shape, value.dtype, value.device
+    if forget.shape != shape or state.shape != shape or (gate is not None and gate.shape != shape):
+        raise ValueError("forget, gate and the state must match value's shape [B, C]")
+    if forget.dtype != dtype or (gate is not None and gate.dtype != dtype):
+        raise ValueError("value, forget and gate must have the same dtype")
+    if forget.device != device or state.device != device or (gate is not None and gate.device != device):
+        raise ValueError("gated step tensors must be on the same device")
+    if out_state is not None and (out_state.shape != shape or out_state.dtype != torch.float32 or out_state.device != device):
         raise ValueError("out_state must be float32 and match the state's shape and device")
     if not value.is_cuda or value.numel() == 0:
-        y, new = _scan_torch(value, forget, gate, state, None) if value.numel() else (value.clone(), state.clone())
-        return y[:, 0], new if out_state is None else out_state.copy_(new)
+        if value.numel() == 0:
+            y, new = value.clone(), state.clone()
+        else:
+            y, new = _scan_torch(value.unsqueeze(1), forget.unsqueeze(1), None if gate is None else gate.unsqueeze(1), state, None)
+            y = y[:, 0]
+        return y, new if out_state is None else out_state.copy_(new)
+    if dtype not in _ACTIVATIONS:
+        raise TypeError(f"unsupported activation dtype {dtype}")
+    if state.dtype != torch.float32:
+        raise ValueError("the state must be float32")
     if torch.is_grad_enabled() and (value.requires_grad or forget.requires_grad or state.requires_grad
                                     or (gate is not None and gate.requires_grad)):
         raise ValueError("gated_step does not support gradients on CUDA; use gated_scan")
-    y = torch.empty(value.shape, device=value.device, dtype=value.dtype)
-    new = torch.empty(state.shape, device=state.device, dtype=torch.float32) if out_state is None else out_state
-    _ext.gated_scan_forward(value, forget, gate, None, state, y=y, out_state=new)
-    return y.squeeze(1), new
+    y = torch.empty(shape, device=device, dtype=dtype)
+    new = torch.empty(shape, device=device, dtype=torch.float32) if out_state is None else out_state
+    _ext.gated_step(value, forget, gate, state, y=y, out_state=new)
+    return y, new
 
 
 class _GatedMixer(nn.Module):
