@@ -11,6 +11,7 @@
 //   G_t = dy_t silu(gate_t) + In_t,            dvalue_t  = G_t (1 - f_t),
 //   dforget_t = G_t (h_{t-1} - value_t) f_t (1 - f_t),   dgate_t = dy_t h_t silu'(gate_t),
 //   dstate_0  = In_0.
+#include <algorithm>
 #include <string>
 
 #include "common.cuh"
@@ -282,7 +283,8 @@ template <typename T, int kTensors, int kThreads, bool kVec> struct Pipeline {
   // repeated: what is left runs through without it.
   __device__ __forceinline__ const T* ready(int64_t i, int64_t t) {
     if constexpr (kVec) {
-      if (ok && t < ntiles) ok = mbar_wait(bars + 8 * (uint32_t)(i & (kStages - 1)), (uint32_t)(i / kStages) & 1u);
+      if (threadIdx.x < 32 && ok && t < ntiles)  // the barrier after it passes it on to the other warps
+        ok = mbar_wait(bars + 8 * (uint32_t)(i & (kStages - 1)), (uint32_t)(i / kStages) & 1u);
     }
     __syncthreads();
     return stage(i);
@@ -675,13 +677,16 @@ cudaError_t launch_tiles(K kernel, const m3_gated_args& a, const Maps& maps, int
                          cudaStream_t stream) {
   const int64_t ntiles = (a.length + kTile - 1) / kTile;
   const int64_t blocks = (int64_t)a.batch * ((a.channels + kChannels - 1) / kChannels);
-  // CTAs that fit the GPU: a cluster takes a sequence's tiles together while its CTAs still have room at once
-  // (past 8 CTAs, a cluster's size without conditions, only where two fit an SM)
+  // A cluster takes a sequence's tiles together while its CTAs still have room on the GPU at once: clusters of up to
+  // 4 in all the room there is (4 x 2048 x 2048: 47 us in fours, 54 in twos), larger ones, whose exchange takes as long
+  // as a tile, up to two CTAs an SM (1 x 65536 x 1536: 317 us in eights, 339 in sixteens; 1 x 32768 x 128: 83 us in
+  // sixteens, 136 in eights). Past 8 CTAs, a cluster's size without conditions, only where two fit an SM.
   const int per_sm = 227 * 1024 / (smem_bytes(tile, tensors, run_maps, 2) + 1024);
-  const int64_t room = (int64_t)sm_count() * per_sm;
   const int most = per_sm > 1 ? kMaxCluster : 8;
   int cluster = 1;
-  while (cluster < most && 2 * cluster <= ntiles && 2 * cluster * blocks <= room) cluster *= 2;
+  while (cluster < most && 2 * cluster <= ntiles &&
+         2 * cluster * blocks <= (int64_t)sm_count() * (cluster < 4 ? per_sm : std::min(per_sm, 2)))
+    cluster *= 2;
   const int smem = smem_bytes(tile, tensors, run_maps, cluster);
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
