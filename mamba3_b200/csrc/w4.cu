@@ -26,18 +26,24 @@ int report_error(int code, const char* msg);
 namespace {
 
 constexpr int kSlab = 128;  // columns that a warp takes at a time, 4 words of 8 codes a thread and output row
-constexpr int kAhead = 2;   // slabs that are under way
 
 // ---- codes ---------------------------------------------------------------------------------------
+
+// (v & mask) | bits, in one instruction
+__device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(bits));
+  return r;
+}
 
 // Two codes to two values code - 8 in T: bytes 0 and 2 of v hold them in their low halves.
 template <typename T> __device__ __forceinline__ uint32_t open2(uint32_t v) {
   if constexpr (std::is_same<T, __half>::value) {
-    const uint32_t w = (v & 0x000F000Fu) | 0x64006400u;
+    const uint32_t w = and_or(v, 0x000F000Fu, 0x64006400u);
     const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&w), __half2half2(__ushort_as_half(0x6408)));
     return *reinterpret_cast<const uint32_t*>(&r);
   } else {
-    const uint32_t w = (v & 0x000F000Fu) | 0x43004300u;
+    const uint32_t w = and_or(v, 0x000F000Fu, 0x43004300u);
     const __nv_bfloat162 r =
         __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&w), __bfloat162bfloat162(__ushort_as_bfloat16(0x4308)));
     return *reinterpret_cast<const uint32_t*>(&r);
@@ -65,98 +71,122 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// N words of one output row from byte `at` on; bytes past the row are 0 (x is 0 there). kAligned: whole words lie
-// on multiples of their size; otherwise, and at the row's end, byte by byte.
-template <bool kAligned, int N>
-__device__ __forceinline__ void load_words(const uint8_t* row, int64_t at, int64_t bytes, int64_t stride, uint32_t* w) {
-  if (kAligned && at + 4 * N <= bytes) {
-    if constexpr (N == 1) {
-      w[0] = __ldcs(reinterpret_cast<const unsigned int*>(row + at));
-    } else if constexpr (N == 2) {
-      const uint2 v = __ldcs(reinterpret_cast<const uint2*>(row + at));
-      w[0] = v.x;
-      w[1] = v.y;
-    } else {
-      const uint4 v = __ldcs(reinterpret_cast<const uint4*>(row + at));
-      w[0] = v.x;
-      w[1] = v.y;
-      w[2] = v.z;
-      w[3] = v.w;
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    w[i] = 0;
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-      if (at + 4 * i + b < bytes) w[i] |= (uint32_t)row[(at + 4 * i + b) * stride] << (8 * b);
-  }
+// A value of a type known at run time, by its bits.
+__device__ __forceinline__ float widen(uint16_t v, bool bf16) {
+  return bf16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
 }
 
 // A warp's 16 output rows, as a thread sees them: rows g and g + 8 (past the end, the last one again: not written).
-template <typename T, int kWords, bool kAligned> struct Weight {
+// kFast: codes in whole aligned words, scales and zeros in 16 bits with unit stride along a row, columns a multiple of
+// 128: read without a check. Otherwise code by code.
+template <typename T, int kWords, bool kFast, bool kZeros> struct Weight {
   static constexpr int kGroup = 32 * kWords, kPerSlab = kSlab / kGroup;
   struct Slab {
     uint32_t code[2][4];
-    float scale[2][kPerSlab], shift[2][kPerSlab];  // s and s (z - 8) of the slab's groups
+    float scale[2][kPerSlab], shift[2][kZeros ? kPerSlab : 1];  // s and z - 8 of the slab's groups
   };
   const m3_w4_args& a;
   const uint8_t* code[2];
-  int64_t scale_at[2], zero_at[2], bytes;
-  int t;
+  const uint16_t *scale[2], *zero[2];
+  int64_t row[2];
+  int t, in_dim, slabs;
 
-  __device__ __forceinline__ Weight(const m3_w4_args& args, int64_t o0, int lane) : a(args), bytes((args.in_dim + 1) / 2), t(lane & 3) {
+  __device__ __forceinline__ Weight(const m3_w4_args& args, int64_t o0, int lane) : a(args), t(lane & 3), in_dim((int)args.in_dim) {
+    slabs = (in_dim + kSlab - 1) / kSlab;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int64_t o = min(o0 + (lane >> 2) + 8 * r, a.out_dim - 1);
-      code[r] = static_cast<const uint8_t*>(a.codes.data) + o * a.codes.stride[0];
-      scale_at[r] = o * a.scales.stride[0];
-      zero_at[r] = o * a.zeros.stride[0];
+      row[r] = min(o0 + (lane >> 2) + 8 * r, a.out_dim - 1);
+      code[r] = static_cast<const uint8_t*>(a.codes.data) + row[r] * a.codes.stride[0] + (kFast ? 4 * kWords * t : 0);
+      if constexpr (kFast) {
+        scale[r] = static_cast<const uint16_t*>(a.scales.data) + row[r] * a.scales.stride[0];
+        if (kZeros) zero[r] = static_cast<const uint16_t*>(a.zeros.data) + row[r] * a.zeros.stride[0];
+      }
     }
   }
   // Pull a slab's codes towards L2.
-  __device__ __forceinline__ void prefetch(int64_t slab) const {
-    const int64_t at = slab * (kSlab / 2) + t * 16;
-    if (at < bytes)
+  __device__ __forceinline__ void prefetch(int slab) const {
+    if (kFast && slab < slabs)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) asm volatile("prefetch.global.L2 [%0];" ::"l"(code[r] + at * a.codes.stride[1]));
+      for (int r = 0; r < 2; ++r) asm volatile("prefetch.global.L2 [%0];" ::"l"(code[r] + slab * (kSlab / 2)));
   }
-  __device__ __forceinline__ void fetch(int64_t slab, Slab& to) const {
+  __device__ __forceinline__ void fetch(int slab, Slab& to) const {
+    if (slab >= slabs) return;
+    if constexpr (kFast) {
+      const bool bf16 = a.scales.dtype == M3_BF16;
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int c = 0; c < kPerSlab; ++c) {
+          const uint8_t* from = code[r] + slab * (kSlab / 2) + c * (kGroup / 2);
+          if constexpr (kWords == 1) {
+            to.code[r][c] = __ldcs(reinterpret_cast<const unsigned int*>(from));
+          } else if constexpr (kWords == 2) {
+            const uint2 v = __ldcs(reinterpret_cast<const uint2*>(from));
+            to.code[r][2 * c] = v.x;
+            to.code[r][2 * c + 1] = v.y;
+          } else {
+            const uint4 v = __ldcs(reinterpret_cast<const uint4*>(from));
+            to.code[r][0] = v.x;
+            to.code[r][1] = v.y;
+            to.code[r][2] = v.z;
+            to.code[r][3] = v.w;
+          }
+          to.scale[r][c] = widen(scale[r][slab * kPerSlab + c], bf16);
+          if (kZeros) to.shift[r][c] = widen(zero[r][slab * kPerSlab + c], bf16) - 8.0f;
+        }
+    } else {
+      careful(slab, to);
+    }
+  }
+  // Any strides, and the end of a row: bytes past it are 0 (x is 0 there), and so are scales.
+  __device__ __forceinline__ void careful(int slab, Slab& to) const {
+    const int bytes = (in_dim + 1) / 2;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const uint8_t* from = static_cast<const uint8_t*>(a.codes.data) + row[r] * a.codes.stride[0];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int at = slab * (kSlab / 2) + w / kWords * (kGroup / 2) + (kWords * t + w % kWords) * 4;
+        uint32_t v = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          if (at + b < bytes) v |= (uint32_t)from[(at + b) * a.codes.stride[1]] << (8 * b);
+        to.code[r][w] = v;
+      }
 #pragma unroll
       for (int c = 0; c < kPerSlab; ++c) {
-        load_words<kAligned, kWords>(code[r], slab * (kSlab / 2) + c * (kGroup / 2) + t * 4 * kWords, bytes, a.codes.stride[1],
-                                     &to.code[r][c * kWords]);
-        const int64_t group = slab * kPerSlab + c;
-        const bool there = group * kGroup < a.in_dim;
-        to.scale[r][c] = there ? ld_t(a.scales, scale_at[r] + group * a.scales.stride[1]) : 0.0f;
-        to.shift[r][c] = there && a.zeros.data ? ld_t(a.zeros, zero_at[r] + group * a.zeros.stride[1]) - 8.0f : 0.0f;
+        const int group = slab * kPerSlab + c;
+        const bool there = group * kGroup < in_dim;
+        to.scale[r][c] = there ? ld_t(a.scales, row[r] * a.scales.stride[0] + group * a.scales.stride[1]) : 0.0f;
+        if (kZeros) to.shift[r][c] = there ? ld_t(a.zeros, row[r] * a.zeros.stride[0] + group * a.zeros.stride[1]) - 8.0f : 0.0f;
       }
+    }
   }
 };
 
 // acc += scale (products - shift sums): the sums of one group, of a thread's 2 x 2 results.
-__device__ __forceinline__ void join(float (&acc)[4], const float (&d)[4], const float (&sums)[4], const float s0, const float s1,
-                                     const float z0, const float z1) {
-  acc[0] = fmaf(s0, fmaf(-z0, sums[0], d[0]), acc[0]);
-  acc[1] = fmaf(s0, fmaf(-z0, sums[1], d[1]), acc[1]);
-  acc[2] = fmaf(s1, fmaf(-z1, sums[0], d[2]), acc[2]);
-  acc[3] = fmaf(s1, fmaf(-z1, sums[1], d[3]), acc[3]);
+template <bool kZeros>
+__device__ __forceinline__ void join(float (&acc)[4], const float (&d)[4], const float (&sums)[4], float s0, float s1, float z0,
+                                     float z1) {
+  acc[0] = fmaf(s0, kZeros ? fmaf(-z0, sums[0], d[0]) : d[0], acc[0]);
+  acc[1] = fmaf(s0, kZeros ? fmaf(-z0, sums[1], d[1]) : d[1], acc[1]);
+  acc[2] = fmaf(s1, kZeros ? fmaf(-z1, sums[0], d[2]) : d[2], acc[2]);
+  acc[3] = fmaf(s1, kZeros ? fmaf(-z1, sums[1], d[3]) : d[3], acc[3]);
 }
 
 // 8 columns of a row of x, from column c on; 0 past the row.
-template <typename T>
-__device__ __forceinline__ uint4 x_unit(const m3_w4_args& a, const T* row, int64_t c, bool units) {
-  if (units && c + 8 <= a.in_dim) return *reinterpret_cast<const uint4*>(row + c);
-  alignas(16) T w[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = c + e < a.in_dim ? row[(c + e) * a.x.stride[1]] : from_f<T>(0.0f);
-  return *reinterpret_cast<const uint4*>(w);
+template <typename T> __device__ __noinline__ uint4 x_careful(const m3_w4_args& a, const T* row, int c) {
+  uint32_t w[4] = {0, 0, 0, 0};
+  for (int e = 0; e < 8; ++e)
+    if (c + e < a.in_dim)
+      w[e >> 1] |= (uint32_t)*reinterpret_cast<const uint16_t*>(row + (c + e) * a.x.stride[1]) << (16 * (e & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T> __device__ __forceinline__ uint4 x_unit(const m3_w4_args& a, const T* row, int c, bool units) {
+  return units && c + 8 <= a.in_dim ? *reinterpret_cast<const uint4*>(row + c) : x_careful(a, row, c);
 }
 
-__device__ __forceinline__ bool x_in_units(const m3_w4_args& a) {
+__host__ __device__ __forceinline__ bool x_in_units(const m3_w4_args& a) {
   return a.x.stride[1] == 1 && a.x.stride[0] % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x.data) & 15) == 0;
 }
 
@@ -165,40 +195,43 @@ __device__ __forceinline__ bool x_in_units(const m3_w4_args& a) {
 // x, a few KB, comes from L1 as the products want it.
 constexpr int kMostWarps = 16;
 
-template <typename T, int kWords, bool kAligned>
+template <typename T, int kWords, bool kFast, bool kZeros>
 __global__ void __launch_bounds__(32 * kMostWarps) w4_few_kernel(const m3_w4_args a) {
-  using W = Weight<T, kWords, kAligned>;
+  using W = Weight<T, kWords, kFast, kZeros>;
+  constexpr int kAhead = 2;  // slabs whose codes are under way
   __shared__ float part[kMostWarps][8][16];
   const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int64_t o0 = (int64_t)blockIdx.x * 16, slabs = (a.in_dim + kSlab - 1) / kSlab;
+  const int64_t o0 = (int64_t)blockIdx.x * 16;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const W weight(a, o0, lane);
   // Launched as a programmatic dependent: what the kernel before wrote, the weight too if it did, is there only after
   // the wait. Until then the first codes are pulled towards L2.
   for (int i = 0; i < kAhead; ++i) weight.prefetch(warp + i * warps);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const bool units = x_in_units(a), here = g < a.rows;
-  const T* row = static_cast<const T*>(a.x.data) + g * a.x.stride[0];
+  const int64_t rows0 = (int64_t)blockIdx.y * 8;
+  const bool units = x_in_units(a), here = rows0 + g < a.rows;
+  const T* row = static_cast<const T*>(a.x.data) + (here ? rows0 + g : 0) * a.x.stride[0];
   typename W::Slab held[kAhead];
-  uint4 x[kAhead][4];
-  auto fetch = [&](int64_t slab, typename W::Slab& w, uint4 (&u)[4]) {
-    if (slab >= slabs) return;
-    weight.fetch(slab, w);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // columns of word i of a thread: group i / kWords of the slab
-      const int64_t c = slab * kSlab + i / kWords * W::kGroup + 8 * (kWords * t + i % kWords);
-      u[i] = here ? x_unit(a, row, c, units) : make_uint4(0u, 0u, 0u, 0u);
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) fetch(warp + i * warps, held[i], x[i]);
+  for (int i = 0; i < kAhead; ++i) weight.fetch(warp + i * warps, held[i]);
   const uint32_t one2 = std::is_same<T, __half>::value ? 0x3C003C00u : 0x3F803F80u;
   float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int64_t slab = warp; slab < slabs; slab += kAhead * warps) {
+  for (int slab0 = warp; slab0 < weight.slabs; slab0 += kAhead * warps) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      if (slab + i * warps >= slabs) break;
+      const int slab = slab0 + i * warps;
+      if (slab >= weight.slabs) break;
+      uint4 x[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {  // columns of word w of a thread: group w / kWords of the slab
+        const int c = slab * kSlab + w / kWords * W::kGroup + 8 * (kWords * t + w % kWords);
+        x[w] = make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (kFast) {
+          if (here) x[w] = *reinterpret_cast<const uint4*>(row + c);
+        } else {
+          if (here) x[w] = x_unit(a, row, c, units);
+        }
+      }
 #pragma unroll
       for (int c = 0; c < W::kPerSlab; ++c) {
         float d[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -207,17 +240,18 @@ __global__ void __launch_bounds__(32 * kMostWarps) w4_few_kernel(const m3_w4_arg
           uint32_t low[4], high[4];
           open8<T>(held[i].code[0][c * kWords + w], low);
           open8<T>(held[i].code[1][c * kWords + w], high);
-          const uint4 b = x[i][c * kWords + w];
+          const uint4 b = x[c * kWords + w];
           mma<T>(d, low[0], high[0], low[1], high[1], b.x, b.y);
           mma<T>(d, low[2], high[2], low[3], high[3], b.z, b.w);
-          if (a.zeros.data) {
+          if (kZeros) {
             mma<T>(sums, one2, one2, one2, one2, b.x, b.y);
             mma<T>(sums, one2, one2, one2, one2, b.z, b.w);
           }
         }
-        join(acc, d, sums, held[i].scale[0][c], held[i].scale[1][c], held[i].shift[0][c], held[i].shift[1][c]);
+        join<kZeros>(acc, d, sums, held[i].scale[0][c], held[i].scale[1][c], held[i].shift[0][kZeros ? c : 0],
+                     held[i].shift[1][kZeros ? c : 0]);
       }
-      fetch(slab + (i + kAhead) * warps, held[i], x[i]);
+      weight.fetch(slab + kAhead * warps, held[i]);
     }
   }
 #pragma unroll
@@ -227,132 +261,302 @@ __global__ void __launch_bounds__(32 * kMostWarps) w4_few_kernel(const m3_w4_arg
   for (int i = threadIdx.x; i < 8 * 16; i += blockDim.x) {
     const int r = i >> 4;
     const int64_t out = o0 + (i & 15);
-    if (r >= a.rows || out >= a.out_dim) continue;
+    if (rows0 + r >= a.rows || out >= a.out_dim) continue;
     float v = 0.0f;
     for (int w = 0; w < warps; ++w) v += part[w][r][i & 15];
-    yp[r * a.y.stride[0] + out * a.y.stride[1]] = from_f<T>(v);
+    yp[(rows0 + r) * a.y.stride[0] + out * a.y.stride[1]] = from_f<T>(v);
   }
 }
 
 // ---- more rows -----------------------------------------------------------------------------------
-// One CTA for 64 outputs and 8 kTiles rows of x: four warps of 16 outputs on even slabs, four on odd ones. x passes
-// through a ring of panels of two slabs in shared memory, which the eight warps share: read by every CTA, it
-// costs more than the codes.
-constexpr int kManyThreads = 256, kPanel = 2 * kSlab, kPanels = 3;
+// The products of many rows are the fifth-generation tensor cores' (the warp-level instruction takes about 27 clocks
+// for 16 x 8 x 16 here: 21 us for the 10768 x 2560 weight at 64 rows). One CTA for 128 outputs and up to kN rows:
+// TMA brings 64 columns of codes and of x a stage, eight warps turn the codes into 16-bit values code - 8 in shared
+// memory (exact); one thread issues the MMAs, which sum one group into one of four accumulators in tensor memory; four warps read
+// it, a thread an output, and add it, scaled, to sums in registers, in float32. Where the outputs are too few for the
+// SMs, a cluster of CTAs shares the columns out and its partial sums meet through distributed shared memory.
+constexpr int kManyOuts = 128, kStage = 64;  // outputs of a CTA, columns of a stage
+constexpr int kStages = 4, kRing = 8;        // of codes as 16-bit values; of codes and x as they come (powers of two)
+constexpr int kProducers = 256, kManyThreads = kProducers + 64 + 128;
+constexpr int kSumsRing = 4;
 
-// A panel's rows of 16-byte units (8 columns). A product reads a unit of each of 8 rows by four threads, group / 32
-// units apart: the rows' pitch, and for groups of 128 a swap of units, spread them over all banks.
-template <int kWords> constexpr int kPitch = kPanel + (kWords == 1 ? 32 : kWords == 2 ? 8 : 16);  // in 16-bit values
-template <int kWords> __device__ __forceinline__ int unit_at(int u) { return kWords == 4 ? u ^ (u >> 3 & 1) : u; }
+template <int kN> struct Many {
+  static constexpr uint32_t kA = kManyOuts * kStage * 2, kX = kN * kStage * 2, kCodes = kManyOuts * kStage / 2;
+  static constexpr uint32_t kOffX = kStages * kA, kOffCodes = kOffX + kRing * kX, kOffBars = kOffCodes + kRing * kCodes;
+  static constexpr uint32_t kOffXSums = kOffBars + 512;  // [groups of this CTA][kN] float: with zero points only
+  static constexpr int kColumns = kSumsRing * kN < 32 ? 32 : kSumsRing * kN;  // of tensor memory
+};
 
-template <typename T, int kWords, bool kAligned, int kTiles>
-__global__ void __launch_bounds__(kManyThreads) w4_many_kernel(const m3_w4_args a) {
-  using W = Weight<T, kWords, kAligned>;
-  constexpr int kRows = 8 * kTiles, kPit = kPitch<kWords>, kUnits = kPanel / 8;
-  extern __shared__ __align__(16) uint8_t smem[];
-  T* xs = reinterpret_cast<T*>(smem);  // [kPanels][kRows][kPit]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, half = warp >> 2;
-  const int64_t o0 = (int64_t)blockIdx.x * 64 + (warp & 3) * 16;
-  const int64_t rows0 = (int64_t)blockIdx.y * kRows;
-  const int rows = (int)min((int64_t)kRows, a.rows - rows0), tiles = (rows + 7) / 8;
-  const int64_t slabs = (a.in_dim + kSlab - 1) / kSlab, panels = (slabs + 1) / 2;
+__device__ __forceinline__ void arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+template <typename T, int kN, bool kZeros>
+__global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_constant__ CUtensorMap x_map, const m3_w4_args a,
+                   int split, bool code_tiles, bool x_tiles) {
+  using M = Many<kN>;
+  extern __shared__ uint8_t raw[];
+  const uint32_t base = (umma::smem_u32(raw) + 1023u) & ~1023u;
+  uint8_t* smem = raw + (base - umma::smem_u32(raw));
+  const uint32_t bars = base + M::kOffBars;
+  auto full = [&](int s) { return bars + 8u * (s & (kStages - 1)); };
+  auto sums_full = [&](int g) { return bars + 8u * (2 * kStages + (g & (kSumsRing - 1))); };
+  auto sums_empty = [&](int g) { return bars + 8u * (2 * kStages + kSumsRing + (g & (kSumsRing - 1))); };
+  auto came = [&](int s) { return bars + 8u * (2 * kStages + 2 * kSumsRing + (s & (kRing - 1))); };
+  auto read = [&](int s) { return bars + 8u * (2 * kStages + 2 * kSumsRing + kRing + (s & (kRing - 1))); };
+  auto freed = [&](int s) { return bars + 8u * (2 * kStages + 2 * kSumsRing + 2 * kRing + (s & (kRing - 1))); };
+  const uint32_t drained = bars + 8u * (2 * kStages + 2 * kSumsRing + 3 * kRing), slot = drained + 8u;
+  float* x_sums = reinterpret_cast<float*>(smem + M::kOffXSums);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int rank = 0;
+  if (split > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int64_t o0 = (int64_t)(blockIdx.x / split) * kManyOuts;
+  const int64_t rows0 = (int64_t)blockIdx.y * kN;
+  const int rows = (int)min((int64_t)kN, a.rows - rows0);
+  const int in_dim = (int)a.in_dim;
+  // this CTA's columns, whole slabs of 128
+  const int slabs = (in_dim + kSlab - 1) / kSlab, per = (slabs + split - 1) / split;
+  const int first = min(in_dim, rank * per * kSlab), last = min(in_dim, (rank + 1) * per * kSlab);
+  const int stages = (last - first + kStage - 1) / kStage, groups = (last - first + a.group - 1) / a.group;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const W weight(a, o0, lane);
-  weight.prefetch(half);
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i)
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(full(i)), "r"(kProducers / 32));
+    for (int i = 0; i < kRing; ++i) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(came(i)));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(read(i)), "r"(kProducers / 32));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(freed(i)));
+    }
+    for (int i = 0; i < kSumsRing; ++i) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(sums_full(i)));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 4;" ::"r"(sums_empty(i)));
+    }
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(drained));
+    asm volatile("fence.mbarrier_init.release.cluster;");
+  }
+  if (warp == kProducers / 32) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(M::kColumns));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  // Launched as a programmatic dependent: what the kernel before wrote, the weight too if it did, is there only after
+  // the wait.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const bool units = x_in_units(a);
   const T* xp = static_cast<const T*>(a.x.data) + rows0 * a.x.stride[0];
-  auto stage = [&](int64_t panel) {
-    if (panel < panels) {
-      T* to = xs + panel % kPanels * kRows * kPit;
-      for (int i = threadIdx.x; i < tiles * 8 * kUnits; i += kManyThreads) {
-        const int r = i / kUnits, u = i % kUnits;
-        const int64_t c = panel * kPanel + 8 * u;
-        T* at = to + r * kPit + 8 * unit_at<kWords>(u);
-        const T* row = xp + (r < rows ? r : 0) * a.x.stride[0];
-        if (units && (c + 8 <= a.in_dim || c >= a.in_dim)) {
-          const bool there = r < rows && c < a.in_dim;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(at))),
-                       "l"(there ? row + c : row), "r"(there ? 16 : 0)
-                       : "memory");
-        } else {
-          *reinterpret_cast<uint4*>(at) = r < rows ? x_unit(a, row, c, false) : make_uint4(0u, 0u, 0u, 0u);
+  if (kZeros) {  // the sums of x over each group, for the zero points
+    for (int i = tid; i < groups * kN; i += kManyThreads) {
+      const int g = i / kN, n = i % kN;
+      float s = 0.0f;
+      if (n < rows)
+        for (int c = first + g * a.group; c < min(last, first + (g + 1) * a.group); c += 8) {
+          const uint4 u = x_unit(a, xp + n * a.x.stride[0], c, units);
+          const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s += to_f(e[j]);
         }
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  for (int i = 0; i < kPanels - 1; ++i) stage(i);
-  typename W::Slab held[kAhead];
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i)
-    if (half + 2 * i < slabs) weight.fetch(half + 2 * i, held[i]);
-  const uint32_t one2 = std::is_same<T, __half>::value ? 0x3C003C00u : 0x3F803F80u;
-  float acc[kTiles][4];
-#pragma unroll
-  for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[n][e] = 0.0f;
-  for (int64_t panel0 = 0; panel0 < panels; panel0 += kAhead) {
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int64_t panel = panel0 + i, slab = 2 * panel + half;
-      if (panel >= panels) break;
-      asm volatile("cp.async.wait_group %0;" ::"n"(kPanels - 2) : "memory");
-      __syncthreads();  // this panel is there, and everyone is done with the one before
-      stage(panel + kPanels - 1);
-      if (slab < slabs) {
-        const T* from = xs + panel % kPanels * kRows * kPit + g * kPit;
-#pragma unroll
-        for (int c = 0; c < W::kPerSlab; ++c) {
-          uint32_t low[kWords][4], high[kWords][4];
-#pragma unroll
-          for (int w = 0; w < kWords; ++w) {
-            open8<T>(held[i].code[0][c * kWords + w], low[w]);
-            open8<T>(held[i].code[1][c * kWords + w], high[w]);
-          }
-#pragma unroll
-          for (int n = 0; n < kTiles; ++n) {
-            if (n >= tiles) break;
-            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int w = 0; w < kWords; ++w) {
-              const uint4 b = *reinterpret_cast<const uint4*>(
-                  from + 8 * n * kPit + 8 * unit_at<kWords>((half * W::kPerSlab + c) * 4 * kWords + t * kWords + w));
-              mma<T>(d, low[w][0], high[w][0], low[w][1], high[w][1], b.x, b.y);
-              mma<T>(d, low[w][2], high[w][2], low[w][3], high[w][3], b.z, b.w);
-              if (a.zeros.data) {
-                mma<T>(sums, one2, one2, one2, one2, b.x, b.y);
-                mma<T>(sums, one2, one2, one2, one2, b.z, b.w);
-              }
-            }
-            join(acc[n], d, sums, held[i].scale[0][c], held[i].scale[1][c], held[i].shift[0][c], held[i].shift[1][c]);
-          }
-        }
-        if (slab + 2 * kAhead < slabs) weight.fetch(slab + 2 * kAhead, held[i]);
-      }
+      x_sums[i] = s;
     }
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  umma::fence_before();
   __syncthreads();
-  float* part = reinterpret_cast<float*>(smem);  // [4][kTiles][4][32]: the odd slabs' sums
-  if (half == 1)
+  umma::fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
+  float acc[kN];  // the consumers' sums
+
+  if (tid < kProducers) {
+    // a thread's part of a stage: 32 columns of one output's codes
+    const int out = tid >> 1, half = tid & 1;
+    const uint8_t* codes = static_cast<const uint8_t*>(a.codes.data) + min(o0 + out, a.out_dim - 1) * a.codes.stride[0];
+    const int bytes = (in_dim + 1) / 2;
+    bool ok = true;
+    for (int s = 0; s < stages; ++s) {
+      uint32_t words[4] = {0, 0, 0, 0};
+      if (ok) ok = umma::mbar_wait(came(s), (uint32_t)(s / kRing) & 1u);
+      if (code_tiles) {
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(words[0]), "=r"(words[1]), "=r"(words[2]), "=r"(words[3])
+                     : "r"(base + M::kOffCodes + (s & (kRing - 1)) * M::kCodes + tid * 16)
+                     : "memory");
+      } else {
+        const int at = (first + s * kStage) / 2 + half * 16;
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n)
+        for (int e = 0; e < 16; ++e)
+          if (at + e < bytes) words[e >> 2] |= (uint32_t)codes[(at + e) * a.codes.stride[1]] << (8 * (e & 3));
+      }
+      // the MMAs of stage s - kStages are done with what this one replaces
+      if (s >= kStages && ok) ok = umma::mbar_wait(freed(s - kStages), (uint32_t)((s - kStages) / kRing) & 1u);
+      if (!x_tiles)
+        for (int i = tid; i < kN * (kStage / 8); i += kProducers) {
+          const int n = i >> 3, u = i & 7, c = first + s * kStage + 8 * u;
+          const uint4 v = n < rows && c < in_dim ? x_unit(a, xp + n * a.x.stride[0], c, units) : make_uint4(0u, 0u, 0u, 0u);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(base + M::kOffX + (s & (kRing - 1)) * M::kX + n * 128 + ((u ^ (n & 7)) << 4)),
+                       "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                       : "memory");
+        }
+      const uint32_t to = base + (s & (kStages - 1)) * M::kA + out * 128;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) part[(((warp & 3) * kTiles + n) * 4 + e) * 32 + lane] = acc[n][e];
-  __syncthreads();
-  if (half == 1) return;
-  T* yp = static_cast<T*>(a.y.data);
-#pragma unroll
-  for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = 8 * n + 2 * t + (e & 1);
-      const int64_t out = o0 + g + 8 * (e >> 1);
-      if (r < rows && out < a.out_dim)
-        yp[(rows0 + r) * a.y.stride[0] + out * a.y.stride[1]] = from_f<T>(acc[n][e] + part[((warp * kTiles + n) * 4 + e) * 32 + lane]);
+      for (int w = 0; w < 4; ++w) {
+        uint32_t v[4];
+        open8<T>(words[w], v);
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + (((4 * half + w) ^ (out & 7)) << 4)), "r"(v[0]), "r"(v[1]),
+                     "r"(v[2]), "r"(v[3])
+                     : "memory");
+      }
+      umma::fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {  // one arrival a warp: a barrier takes them one by one
+        arrive(full(s));
+        arrive(read(s));
+      }
     }
+  } else if (warp == kProducers / 32 + 1) {
+    if (lane == 0) {  // the copies; a stage's barrier completes without bytes where TMA cannot read either
+      bool ok = true;
+      int s = 0;
+      for (; s < stages && ok; ++s) {
+        if (s >= kRing) {
+          ok = umma::mbar_wait(read(s), (uint32_t)(s / kRing - 1) & 1u);
+          if (ok) ok = umma::mbar_wait(freed(s), (uint32_t)(s / kRing - 1) & 1u);  // the MMAs are done with its x
+          if (!ok) break;
+        }
+        umma::mbar_expect_tx(came(s), (code_tiles ? M::kCodes : 0) + (x_tiles ? M::kX : 0));
+        const int c = first + s * kStage;
+        if (code_tiles)
+          asm volatile(
+              "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+                  base + M::kOffCodes + (s & (kRing - 1)) * M::kCodes),
+              "l"(reinterpret_cast<uint64_t>(&code_map)), "r"(c / 2), "r"((int)o0), "r"(came(s))
+              : "memory");
+        if (x_tiles)
+          asm volatile(
+              "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+                  base + M::kOffX + (s & (kRing - 1)) * M::kX),
+              "l"(reinterpret_cast<uint64_t>(&x_map)), "r"(c), "r"((int)rows0), "r"(came(s))
+              : "memory");
+      }
+      if (!ok)  // gave up: the copies under way land before the block's shared memory goes
+        for (int i = max(0, s - kRing); i < s; ++i) umma::mbar_wait(came(i), (uint32_t)(i / kRing) & 1u);
+    }
+  } else if (warp == kProducers / 32) {
+    if (lane == 0) {
+      const uint32_t id = umma::idesc(kManyOuts, kN, std::is_same<T, __nv_bfloat16>::value, false, false);
+      const uint64_t da0 = umma::sdesc(base, 16, 1024), db0 = umma::sdesc(base + M::kOffX, 16, 1024);
+      // This one thread's instructions are the chain that all else waits for: no division, one commit a stage and one a
+      // group. A stage is a group's half, a group or two; columns past the row are zeros of x.
+      const int parts = a.group == 32 ? 2 : 1, stages_of = a.group == 128 ? 2 : 1;
+      bool ok = true;
+      int g = 0;
+      for (int s = 0; s < stages && ok; ++s) {
+        ok = umma::mbar_wait(full(s), (uint32_t)(s / kStages) & 1u);
+        if (!ok) break;
+        umma::fence_after();
+        const uint64_t da = umma::sdesc_at(da0, (s & (kStages - 1)) * M::kA), db = umma::sdesc_at(db0, (s & (kRing - 1)) * M::kX);
+        const bool opens = stages_of == 1 || (s & 1) == 0, closes = stages_of == 1 || (s & 1) == 1 || s + 1 == stages;
+        auto begin = [&]() { return g < kSumsRing || umma::mbar_wait(sums_empty(g), (uint32_t)(g / kSumsRing - 1) & 1u); };
+        if (opens) ok = begin();
+        if (!ok) break;
+        uint32_t to = tmem + (g & (kSumsRing - 1)) * kN;
+        umma::mma_f16(to, da, db, id, !opens);
+        umma::mma_f16(to, umma::sdesc_at(da, 32), umma::sdesc_at(db, 32), id, 1);
+        if (parts == 2) {
+          umma::mma_commit(sums_full(g));
+          if (++g == groups) {
+            umma::mma_commit(freed(s));
+            break;
+          }
+          ok = begin();
+          if (!ok) break;
+          to = tmem + (g & (kSumsRing - 1)) * kN;
+        }
+        umma::mma_f16(to, umma::sdesc_at(da, 64), umma::sdesc_at(db, 64), id, parts == 1);
+        umma::mma_f16(to, umma::sdesc_at(da, 96), umma::sdesc_at(db, 96), id, 1);
+        if (closes) umma::mma_commit(sums_full(g++));
+        umma::mma_commit(freed(s));
+      }
+      if (!ok) {  // the MMAs issued so far end before their memory is given back
+        umma::mma_commit(drained);
+        umma::mbar_wait(drained, 0);
+      }
+    }
+  } else {
+    const int quarter = warp & 3, out = quarter * 32 + lane;
+    const int64_t o = min(o0 + out, a.out_dim - 1);
+    const int64_t scale_at = o * a.scales.stride[0], zero_at = o * a.zeros.stride[0];
+#pragma unroll
+    for (int n = 0; n < kN; ++n) acc[n] = 0.0f;
+    auto value = [&](const m3_tensor& t, int64_t at, int g) { return g < groups ? ld_t(t, at + (first / a.group + g) * t.stride[1]) : 0.0f; };
+    float s_next = value(a.scales, scale_at, 0), z_next = kZeros ? value(a.zeros, zero_at, 0) : 0.0f;
+    bool ok = true;
+    for (int g = 0; g < groups; ++g) {
+      const float s = s_next, z = z_next - 8.0f;
+      s_next = value(a.scales, scale_at, g + 1);
+      if (kZeros) z_next = value(a.zeros, zero_at, g + 1);
+      ok = __all_sync(0xffffffffu, umma::mbar_wait(sums_full(g), (uint32_t)(g / kSumsRing) & 1u));
+      if (!ok) break;
+      umma::fence_after();
+#pragma unroll
+      for (int n0 = 0; n0 < kN; n0 += 16) {
+        uint32_t r[16];
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+              "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+            : "r"(tmem + (g & (kSumsRing - 1)) * kN + n0 + ((uint32_t)(quarter * 32) << 16)));
+        umma::tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float d = __uint_as_float(r[e]);
+          acc[n0 + e] = fmaf(s, kZeros ? fmaf(-z, x_sums[g * kN + n0 + e], d) : d, acc[n0 + e]);
+        }
+      }
+      umma::fence_before();
+      __syncwarp();
+      if (lane == 0) arrive(sums_empty(g));
+    }
+  }
+  __syncwarp();
+  umma::fence_before();
+  __syncthreads();
+  umma::fence_after();
+  if (warp == kProducers / 32)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(M::kColumns));
+  T* yp = static_cast<T*>(a.y.data);
+  const int out = (warp & 3) * 32 + lane;
+  const bool consumer = warp > kProducers / 32 + 1;
+  if (split == 1) {
+    if (consumer && o0 + out < a.out_dim) {
+#pragma unroll
+      for (int n = 0; n < kN; ++n)
+        if (n < rows) yp[(rows0 + n) * a.y.stride[0] + (o0 + out) * a.y.stride[1]] = from_f<T>(acc[n]);
+    }
+    return;
+  }
+  // the cluster's partial sums: [kN][128] in every CTA's shared memory; CTA r adds up rows r kN / split ...
+  float* part = reinterpret_cast<float*>(smem);
+  if (consumer) {
+#pragma unroll
+    for (int n = 0; n < kN; ++n) part[n * kManyOuts + out] = acc[n];
+  }
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  const int share = kN / split;
+  for (int i = tid; i < share * kManyOuts; i += kManyThreads) {
+    const int n = rank * share + i / kManyOuts, oo = i % kManyOuts;
+    float v = 0.0f;
+    for (int r = 0; r < split; ++r) {
+      uint32_t at;
+      float p;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(umma::smem_u32(part + n * kManyOuts + oo)), "r"(r));
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(p) : "r"(at) : "memory");
+      v += p;
+    }
+    if (n < rows && o0 + oo < a.out_dim) yp[(rows0 + n) * a.y.stride[0] + (o0 + oo) * a.y.stride[1]] = from_f<T>(v);
+  }
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // no CTA leaves while another reads its sums
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // ---- host ----------------------------------------------------------------------------------------
@@ -370,40 +574,81 @@ cudaLaunchConfig_t config(dim3 grid, int threads, size_t smem, cudaStream_t stre
   return cfg;
 }
 
-template <typename T, int kWords, bool kAligned, int kTiles> cudaError_t launch_many(const m3_w4_args& a, cudaStream_t stream) {
-  constexpr size_t smem = (size_t)kPanels * 8 * kTiles * kPitch<kWords> * 2;
-  static_assert(smem >= 4 * kTiles * 4 * 32 * 4, "the odd slabs' sums fit the panels");
-  auto kernel = w4_many_kernel<T, kWords, kAligned, kTiles>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return e;
-  cudaLaunchAttribute chained;
-  const dim3 grid((unsigned)((a.out_dim + 63) / 64), (unsigned)((a.rows + 8 * kTiles - 1) / (8 * kTiles)));
-  const cudaLaunchConfig_t cfg = config(grid, kManyThreads, smem, stream, &chained);
-  return cudaLaunchKernelEx(&cfg, kernel, a);
+// Boxes of box_cols x box_rows of a matrix; what lies outside reads as 0.
+bool encode(CUtensorMap* map, CUtensorMapDataType type, const m3_tensor& t, int64_t cols, int64_t rows, int elem, int box_cols,
+            int box_rows, CUtensorMapSwizzle swizzle) {
+  const PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+  if (enc == nullptr) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(rows == 1 ? (cols * elem + 15) / 16 * 16 : t.stride[0] * elem)};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, step[2] = {1, 1};
+  return enc(map, type, 2, t.data, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int kWords, bool kAligned> cudaError_t launch_rows(const m3_w4_args& a, cudaStream_t stream) {
-  if (a.rows <= 8) {
-    // warps for the columns of 16 outputs: enough to give every SM 16, while each has two slabs or more
-    const int64_t tiles = (a.out_dim + 15) / 16, slabs = (a.in_dim + kSlab - 1) / kSlab;
-    int warps = 4;
-    while (warps < kMostWarps && tiles * warps < (int64_t)16 * sm_count() && 4 * warps <= slabs) warps *= 2;
-    cudaLaunchAttribute chained;
-    const cudaLaunchConfig_t cfg = config(dim3((unsigned)tiles), 32 * warps, 0, stream, &chained);
-    return cudaLaunchKernelEx(&cfg, w4_few_kernel<T, kWords, kAligned>, a);
+// (false: the sums of x of a very long row do not fit shared memory)
+template <typename T, int kN, bool kZeros> bool launch_many(const m3_w4_args& a, cudaStream_t stream, cudaError_t* e) {
+  // CTAs for the columns of 128 outputs: while that leaves SMs idle and each has four slabs or more
+  const int64_t tiles = (a.out_dim + kManyOuts - 1) / kManyOuts, slabs = (a.in_dim + kSlab - 1) / kSlab;
+  const int64_t row_tiles = (a.rows + kN - 1) / kN;
+  int split = 1;
+  while (split < 8 && 2 * split * tiles * row_tiles <= sm_count() && slabs >= 8 * split) split *= 2;
+  const int64_t groups = (slabs + split - 1) / split * (kSlab / a.group);
+  const size_t smem = 1024 + std::max<size_t>(Many<kN>::kOffXSums + (kZeros ? groups * kN * 4 : 0), (size_t)kN * kManyOuts * 4);
+  if (smem > 227 * 1024) return false;
+  auto kernel = w4_many_kernel<T, kN, kZeros>;
+  *e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (*e != cudaSuccess) return true;
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = config(dim3((unsigned)(tiles * split), (unsigned)row_tiles), kManyThreads, smem, stream, attr);
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.numAttrs = split > 1 ? 2 : 1;
+  const bool code_tiles = a.codes.stride[1] == 1 && (a.codes.stride[0] > 0 || a.out_dim == 1) && a.codes.stride[0] % 16 == 0 &&
+                          reinterpret_cast<uintptr_t>(a.codes.data) % 16 == 0;
+  const bool x_tiles = x_in_units(a) && a.x.stride[0] > 0;
+  CUtensorMap code_map = {}, x_map = {};
+  if ((code_tiles && !encode(&code_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, (a.in_dim + 1) / 2, a.out_dim, 1, kStage / 2,
+                             kManyOuts, CU_TENSOR_MAP_SWIZZLE_NONE)) ||
+      (x_tiles && !encode(&x_map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                          a.x, a.in_dim, a.rows, 2, kStage, kN, CU_TENSOR_MAP_SWIZZLE_128B))) {
+    *e = cudaErrorInvalidValue;
+    return true;
   }
-  if (a.rows <= 16) return launch_many<T, kWords, kAligned, 2>(a, stream);
-  if (a.rows <= 32) return launch_many<T, kWords, kAligned, 4>(a, stream);
-  return launch_many<T, kWords, kAligned, 8>(a, stream);  // past 64 rows, the weight is read once for every 64
+  *e = cudaLaunchKernelEx(&cfg, kernel, code_map, x_map, a, split, code_tiles, x_tiles);
+  return true;
+}
+
+// Past 64 rows, the weight is read once for every 64.
+template <typename T, bool kZeros> bool launch_many_rows(const m3_w4_args& a, cudaStream_t stream, cudaError_t* e) {
+  if (a.rows > 32 && launch_many<T, 64, kZeros>(a, stream, e)) return true;
+  if (a.rows > 16 && launch_many<T, 32, kZeros>(a, stream, e)) return true;
+  return launch_many<T, 16, kZeros>(a, stream, e);
+}
+
+template <typename T, int kWords, bool kFast, bool kZeros> cudaError_t launch_few(const m3_w4_args& a, cudaStream_t stream) {
+  // warps for the columns of 16 outputs: enough to give every SM 16, while each has two slabs or more
+  const int64_t tiles = (a.out_dim + 15) / 16, slabs = (a.in_dim + kSlab - 1) / kSlab;
+  int warps = 4;
+  while (warps < kMostWarps && tiles * warps < (int64_t)16 * sm_count() && 4 * warps <= slabs) warps *= 2;
+  cudaLaunchAttribute chained;
+  const cudaLaunchConfig_t cfg = config(dim3((unsigned)tiles, (unsigned)((a.rows + 7) / 8)), 32 * warps, 0, stream, &chained);
+  return cudaLaunchKernelEx(&cfg, w4_few_kernel<T, kWords, kFast, kZeros>, a);
 }
 
 template <typename T, int kWords> cudaError_t launch_group(const m3_w4_args& a, cudaStream_t stream) {
-  const bool aligned = a.codes.stride[1] == 1 && a.codes.stride[0] % (4 * kWords) == 0 &&
-                       reinterpret_cast<uintptr_t>(a.codes.data) % (4 * kWords) == 0;
-  return aligned ? launch_rows<T, kWords, true>(a, stream) : launch_rows<T, kWords, false>(a, stream);
+  const bool fast = a.codes.stride[1] == 1 && a.codes.stride[0] % (4 * kWords) == 0 &&
+                    reinterpret_cast<uintptr_t>(a.codes.data) % (4 * kWords) == 0 && a.scales.dtype != M3_F32 && x_in_units(a) &&
+                    a.in_dim % kSlab == 0 &&
+                    a.scales.stride[1] == 1 && (a.zeros.data == nullptr || a.zeros.stride[1] == 1);
+  if (a.zeros.data) return fast ? launch_few<T, kWords, true, true>(a, stream) : launch_few<T, kWords, false, true>(a, stream);
+  return fast ? launch_few<T, kWords, true, false>(a, stream) : launch_few<T, kWords, false, false>(a, stream);
 }
 
 template <typename T> cudaError_t launch_type(const m3_w4_args& a, cudaStream_t stream) {
+  cudaError_t e = cudaSuccess;
+  if (a.rows > 8 && (a.zeros.data ? launch_many_rows<T, true>(a, stream, &e) : launch_many_rows<T, false>(a, stream, &e))) return e;
   switch (a.group) {
     case 32: return launch_group<T, 1>(a, stream);
     case 64: return launch_group<T, 2>(a, stream);

@@ -68,12 +68,19 @@ def test_model_sizes_and_float32_scales(shape):
         _check(x, codes, scales, zero, 128, y)
 
 
+def test_very_long_rows():
+    """More groups than the many-row kernel has shared memory for the sums of x."""
+    codes, scales, zero = _weight(20, 120000, 32, True, torch.float16)
+    x = torch.randn(18, 120000, device="cuda").to(torch.float16)
+    _check(x, codes, scales, zero, 32, linear_w4(x, codes, scales, zero, group_size=32))
+
+
 def test_strides_and_offsets():
     codes, scales, zero = _weight(96, 256, 32, True, torch.bfloat16)
     wide = torch.randn(6, 515, device="cuda").to(torch.bfloat16)
     wide_codes = torch.zeros(96, 200, device="cuda", dtype=torch.uint8)
     wide_codes[:, 3:131] = codes
-    for x in (wide[:, :256], wide[:, 1:257], wide[::2, 3:259], wide.t().contiguous().t()[:, :256], wide[:1].expand(6, -1)[:, :256]):
+    for x in (wide[:, :256], wide[:, :256].repeat(5, 1), wide[:, 1:257].repeat(4, 1)[::2], wide[:, 1:257], wide[::2, 3:259], wide.t().contiguous().t()[:, :256], wide[:1].expand(6, -1)[:, :256]):
         for q in (codes, wide_codes[:, 3:131], codes.t().contiguous().t()):
             for s in (scales, scales.t().contiguous().t()):
                 _check(x, q, s, zero, 32, linear_w4(x, q, s, zero, group_size=32))
