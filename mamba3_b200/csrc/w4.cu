@@ -71,6 +71,31 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// kCount words of a row of codes from byte `at` on, any strides and alignment; bytes past the row are 0. Inside the row
+// they come as aligned words, shifted into place.
+template <int kCount>
+__device__ __forceinline__ void row_words(const uint8_t* row, int64_t step, int at, int bytes, uint32_t* to) {
+  if (step == 1 && at >= 4 && at + 4 * kCount + 4 <= bytes) {
+    const uint8_t* from = row + at;
+    const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(from) & 3);
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(from - off);
+    uint32_t held[kCount + 1];
+#pragma unroll
+    for (int i = 0; i <= kCount; ++i) held[i] = words[i];
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) to[i] = __funnelshift_r(held[i], held[i + 1], 8 * off);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      uint32_t v = 0;
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        if (at + 4 * i + b < bytes) v |= (uint32_t)row[(at + 4 * i + b) * step] << (8 * b);
+      to[i] = v;
+    }
+  }
+}
+
 // A value of a type known at run time, by its bits.
 __device__ __forceinline__ float widen(uint16_t v, bool bf16) {
   return bf16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
@@ -145,14 +170,8 @@ template <typename T, int kWords, bool kFast, bool kZeros> struct Weight {
     for (int r = 0; r < 2; ++r) {
       const uint8_t* from = static_cast<const uint8_t*>(a.codes.data) + row[r] * a.codes.stride[0];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const int at = slab * (kSlab / 2) + w / kWords * (kGroup / 2) + (kWords * t + w % kWords) * 4;
-        uint32_t v = 0;
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-          if (at + b < bytes) v |= (uint32_t)from[(at + b) * a.codes.stride[1]] << (8 * b);
-        to.code[r][w] = v;
-      }
+      for (int c = 0; c < kPerSlab; ++c)
+        row_words<kWords>(from, a.codes.stride[1], slab * (kSlab / 2) + c * (kGroup / 2) + 4 * kWords * t, bytes, to.code[r] + c * kWords);
 #pragma unroll
       for (int c = 0; c < kPerSlab; ++c) {
         const int group = slab * kPerSlab + c;
@@ -177,6 +196,11 @@ __device__ __forceinline__ void join(float (&acc)[4], const float (&d)[4], const
 // 8 columns of a row of x, from column c on; 0 past the row.
 template <typename T> __device__ __noinline__ uint4 x_careful(const m3_w4_args& a, const T* row, int c) {
   uint32_t w[4] = {0, 0, 0, 0};
+  if (a.x.stride[1] == 1 && c + 8 <= a.in_dim) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[c + e] << (16 * (e & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
   for (int e = 0; e < 8; ++e)
     if (c + e < a.in_dim)
       w[e >> 1] |= (uint32_t)*reinterpret_cast<const uint16_t*>(row + (c + e) * a.x.stride[1]) << (16 * (e & 1));
@@ -187,7 +211,7 @@ template <typename T> __device__ __forceinline__ uint4 x_unit(const m3_w4_args& 
 }
 
 __host__ __device__ __forceinline__ bool x_in_units(const m3_w4_args& a) {
-  return a.x.stride[1] == 1 && a.x.stride[0] % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x.data) & 15) == 0;
+  return a.x.stride[1] == 1 && (a.rows == 1 || a.x.stride[0] % 8 == 0) && (reinterpret_cast<uintptr_t>(a.x.data) & 15) == 0;
 }
 
 // ---- up to 8 rows --------------------------------------------------------------------------------
@@ -208,9 +232,8 @@ __global__ void __launch_bounds__(32 * kMostWarps) w4_few_kernel(const m3_w4_arg
   // the wait. Until then the first codes are pulled towards L2.
   for (int i = 0; i < kAhead; ++i) weight.prefetch(warp + i * warps);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t rows0 = (int64_t)blockIdx.y * 8;
-  const bool units = x_in_units(a), here = rows0 + g < a.rows;
-  const T* row = static_cast<const T*>(a.x.data) + (here ? rows0 + g : 0) * a.x.stride[0];
+  const bool units = x_in_units(a), here = g < a.rows;
+  const T* row = static_cast<const T*>(a.x.data) + (here ? g : 0) * a.x.stride[0];
   typename W::Slab held[kAhead];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) weight.fetch(warp + i * warps, held[i]);
@@ -261,10 +284,10 @@ __global__ void __launch_bounds__(32 * kMostWarps) w4_few_kernel(const m3_w4_arg
   for (int i = threadIdx.x; i < 8 * 16; i += blockDim.x) {
     const int r = i >> 4;
     const int64_t out = o0 + (i & 15);
-    if (rows0 + r >= a.rows || out >= a.out_dim) continue;
+    if (r >= a.rows || out >= a.out_dim) continue;
     float v = 0.0f;
     for (int w = 0; w < warps; ++w) v += part[w][r][i & 15];
-    yp[(rows0 + r) * a.y.stride[0] + out * a.y.stride[1]] = from_f<T>(v);
+    yp[r * a.y.stride[0] + out * a.y.stride[1]] = from_f<T>(v);
   }
 }
 
@@ -277,22 +300,46 @@ __global__ void __launch_bounds__(32 * kMostWarps) w4_few_kernel(const m3_w4_arg
 // SMs, a cluster of CTAs shares the columns out and its partial sums meet through distributed shared memory.
 constexpr int kManyOuts = 128, kStage = 64;  // outputs of a CTA, columns of a stage
 constexpr int kStages = 4, kRing = 8;        // of codes as 16-bit values; of codes and x as they come (powers of two)
-constexpr int kProducers = 256, kManyThreads = kProducers + 64 + 128;
+constexpr int kTeams = 3, kProducers = 128 * kTeams, kManyThreads = kProducers + 64 + 128;
 constexpr int kSumsRing = 4;
 
 template <int kN> struct Many {
   static constexpr uint32_t kA = kManyOuts * kStage * 2, kX = kN * kStage * 2, kCodes = kManyOuts * kStage / 2;
   static constexpr uint32_t kOffX = kStages * kA, kOffCodes = kOffX + kRing * kX, kOffBars = kOffCodes + kRing * kCodes;
-  static constexpr uint32_t kOffXSums = kOffBars + 512;  // [groups of this CTA][kN] float: with zero points only
-  static constexpr int kColumns = kSumsRing * kN < 32 ? 32 : kSumsRing * kN;  // of tensor memory
+  static constexpr uint32_t kOffOnes = kOffBars + 1024;  // a tile of ones, with zero points only
+  static constexpr uint32_t kBytes = 1024 + std::max<uint32_t>(kOffOnes, kN * kManyOuts * 4);  // without the ones
+  static constexpr int kColumns = 2 * kSumsRing * kN;  // of tensor memory: products, and sums of x where there are zero points
 };
 
 __device__ __forceinline__ void arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+__device__ __forceinline__ void mma_if(uint32_t leader, uint32_t to, uint64_t da, uint64_t db, uint32_t id, uint32_t adds) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(to),
+      "l"(da), "l"(db), "r"(id), "r"(adds), "r"(leader));
+}
+__device__ __forceinline__ void commit_if(uint32_t leader, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(bar),
+      "r"(leader)
+      : "memory");
+}
+
+__device__ __forceinline__ void load16(uint32_t from, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(from));
+}
+
 template <typename T, int kN, bool kZeros>
-__global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_constant__ CUtensorMap x_map, const m3_w4_args a,
+__global__ void __launch_bounds__(kManyThreads, 1)
+    w4_many_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_constant__ CUtensorMap x_map, const m3_w4_args a,
                    int split, bool code_tiles, bool x_tiles) {
   using M = Many<kN>;
   extern __shared__ uint8_t raw[];
@@ -306,8 +353,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(const __grid_c
   auto read = [&](int s) { return bars + 8u * (2 * kStages + 2 * kSumsRing + kRing + (s & (kRing - 1))); };
   auto freed = [&](int s) { return bars + 8u * (2 * kStages + 2 * kSumsRing + 2 * kRing + (s & (kRing - 1))); };
   const uint32_t drained = bars + 8u * (2 * kStages + 2 * kSumsRing + 3 * kRing), slot = drained + 8u;
-  float* x_sums = reinterpret_cast<float*>(smem + M::kOffXSums);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   int rank = 0;
   if (split > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   const int64_t o0 = (int64_t)(blockIdx.x / split) * kManyOuts;
@@ -321,10 +367,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(const __grid_c
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i)
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(full(i)), "r"(kProducers / 32));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(full(i)), "r"(4));
     for (int i = 0; i < kRing; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(came(i)));
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(read(i)), "r"(kProducers / 32));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(read(i)), "r"(4));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(freed(i)));
     }
     for (int i = 0; i < kSumsRing; ++i) {
@@ -343,19 +389,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(const __grid_c
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const bool units = x_in_units(a);
   const T* xp = static_cast<const T*>(a.x.data) + rows0 * a.x.stride[0];
-  if (kZeros) {  // the sums of x over each group, for the zero points
-    for (int i = tid; i < groups * kN; i += kManyThreads) {
-      const int g = i / kN, n = i % kN;
-      float s = 0.0f;
-      if (n < rows)
-        for (int c = first + g * a.group; c < min(last, first + (g + 1) * a.group); c += 8) {
-          const uint4 u = x_unit(a, xp + n * a.x.stride[0], c, units);
-          const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) s += to_f(e[j]);
-        }
-      x_sums[i] = s;
-    }
+  if (kZeros) {
+    const uint32_t one2 = std::is_same<T, __half>::value ? 0x3C003C00u : 0x3F803F80u;
+    for (int i = tid; i < (int)M::kA / 16; i += kManyThreads)
+      asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(base + M::kOffOnes + 16 * i), "r"(one2) : "memory");
+    umma::fence_async_smem();
   }
   umma::fence_before();
   __syncthreads();
@@ -365,29 +403,27 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(const __grid_c
   float acc[kN];  // the consumers' sums
 
   if (tid < kProducers) {
-    // a thread's part of a stage: 32 columns of one output's codes
-    const int out = tid >> 1, half = tid & 1;
+    // the teams take stages in turn; a thread's part of one is the 64 columns of an output
+    const int out = tid & 127, flip = (out >> 2) & 1;  // (the copy's 32-byte swizzle: halves change places every four rows)
     const uint8_t* codes = static_cast<const uint8_t*>(a.codes.data) + min(o0 + out, a.out_dim - 1) * a.codes.stride[0];
-    const int bytes = (in_dim + 1) / 2;
     bool ok = true;
-    for (int s = 0; s < stages; ++s) {
-      uint32_t words[4] = {0, 0, 0, 0};
+    for (int s = tid >> 7; s < stages; s += kTeams) {
+      uint32_t words[8];
+      if (!code_tiles) row_words<8>(codes, a.codes.stride[1], (first + s * kStage) / 2, (in_dim + 1) / 2, words);
       if (ok) ok = umma::mbar_wait(came(s), (uint32_t)(s / kRing) & 1u);
       if (code_tiles) {
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(words[0]), "=r"(words[1]), "=r"(words[2]), "=r"(words[3])
-                     : "r"(base + M::kOffCodes + (s & (kRing - 1)) * M::kCodes + tid * 16)
-                     : "memory");
-      } else {
-        const int at = (first + s * kStage) / 2 + half * 16;
+        const uint32_t from = base + M::kOffCodes + (s & (kRing - 1)) * M::kCodes + out * 32;
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (at + e < bytes) words[e >> 2] |= (uint32_t)codes[(at + e) * a.codes.stride[1]] << (8 * (e & 3));
+        for (int h = 0; h < 2; ++h)
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(words[4 * h]), "=r"(words[4 * h + 1]), "=r"(words[4 * h + 2]), "=r"(words[4 * h + 3])
+                       : "r"(from + ((h ^ flip) << 4))
+                       : "memory");
       }
       // the MMAs of stage s - kStages are done with what this one replaces
       if (s >= kStages && ok) ok = umma::mbar_wait(freed(s - kStages), (uint32_t)((s - kStages) / kRing) & 1u);
       if (!x_tiles)
-        for (int i = tid; i < kN * (kStage / 8); i += kProducers) {
+        for (int i = out; i < kN * (kStage / 8); i += 128) {
           const int n = i >> 3, u = i & 7, c = first + s * kStage + 8 * u;
           const uint4 v = n < rows && c < in_dim ? x_unit(a, xp + n * a.x.stride[0], c, units) : make_uint4(0u, 0u, 0u, 0u);
           asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(base + M::kOffX + (s & (kRing - 1)) * M::kX + n * 128 + ((u ^ (n & 7)) << 4)),
@@ -396,11 +432,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(const __grid_c
         }
       const uint32_t to = base + (s & (kStages - 1)) * M::kA + out * 128;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < 8; ++w) {
         uint32_t v[4];
         open8<T>(words[w], v);
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + (((4 * half + w) ^ (out & 7)) << 4)), "r"(v[0]), "r"(v[1]),
-                     "r"(v[2]), "r"(v[3])
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + ((w ^ (out & 7)) << 4)), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                     "r"(v[3])
                      : "memory");
       }
       umma::fence_async_smem();
@@ -439,46 +475,52 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(const __grid_c
         for (int i = max(0, s - kRing); i < s; ++i) umma::mbar_wait(came(i), (uint32_t)(i / kRing) & 1u);
     }
   } else if (warp == kProducers / 32) {
-    if (lane == 0) {
-      const uint32_t id = umma::idesc(kManyOuts, kN, std::is_same<T, __nv_bfloat16>::value, false, false);
-      const uint64_t da0 = umma::sdesc(base, 16, 1024), db0 = umma::sdesc(base + M::kOffX, 16, 1024);
-      // This one thread's instructions are the chain that all else waits for: no division, one commit a stage and one a
-      // group. A stage is a group's half, a group or two; columns past the row are zeros of x.
-      const int parts = a.group == 32 ? 2 : 1, stages_of = a.group == 128 ? 2 : 1;
-      bool ok = true;
-      int g = 0;
-      for (int s = 0; s < stages && ok; ++s) {
-        ok = umma::mbar_wait(full(s), (uint32_t)(s / kStages) & 1u);
+    // The chain that all else waits for: no division, one commit a stage and one a group. The whole warp goes through
+    // it and one lane's instructions count, so that addresses and descriptors are the warp's, in uniform registers.
+    uint32_t leader;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+    const uint32_t id = umma::idesc(kManyOuts, kN, std::is_same<T, __nv_bfloat16>::value, false, false);
+    const uint32_t acc0 = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint64_t da0 = umma::sdesc(base, 16, 1024), db0 = umma::sdesc(base + M::kOffX, 16, 1024);
+    const uint64_t ones = umma::sdesc(base + M::kOffOnes, 16, 1024);
+    auto product = [&](uint32_t to, uint64_t da, uint64_t db, uint32_t adds) {
+      mma_if(leader, to, da, db, id, adds);
+      if (kZeros) mma_if(leader, to + kSumsRing * kN, ones, db, id, adds);  // the sums of x, the same for every output
+    };
+    // A stage is half a group, a group or two; columns past the row are zeros of x.
+    const int parts = a.group == 32 ? 2 : 1, stages_of = a.group == 128 ? 2 : 1;
+    bool ok = true;
+    int g = 0;
+    for (int s = 0; s < stages && ok; ++s) {
+      ok = umma::mbar_wait(full(s), (uint32_t)(s / kStages) & 1u);
+      auto begin = [&]() { return g < kSumsRing || umma::mbar_wait(sums_empty(g), (uint32_t)(g / kSumsRing - 1) & 1u); };
+      const bool opens = stages_of == 1 || (s & 1) == 0, closes = stages_of == 1 || (s & 1) == 1 || s + 1 == stages;
+      if (opens) ok = ok && begin();
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      umma::fence_after();
+      const uint64_t da = umma::sdesc_at(da0, (s & (kStages - 1)) * M::kA), db = umma::sdesc_at(db0, (s & (kRing - 1)) * M::kX);
+      uint32_t to = acc0 + (g & (kSumsRing - 1)) * kN;
+      product(to, da, db, !opens);
+      product(to, umma::sdesc_at(da, 32), umma::sdesc_at(db, 32), 1);
+      if (parts == 2) {
+        commit_if(leader, sums_full(g));
+        if (++g == groups) {
+          commit_if(leader, freed(s));
+          break;
+        }
+        ok = __all_sync(0xffffffffu, begin());
         if (!ok) break;
         umma::fence_after();
-        const uint64_t da = umma::sdesc_at(da0, (s & (kStages - 1)) * M::kA), db = umma::sdesc_at(db0, (s & (kRing - 1)) * M::kX);
-        const bool opens = stages_of == 1 || (s & 1) == 0, closes = stages_of == 1 || (s & 1) == 1 || s + 1 == stages;
-        auto begin = [&]() { return g < kSumsRing || umma::mbar_wait(sums_empty(g), (uint32_t)(g / kSumsRing - 1) & 1u); };
-        if (opens) ok = begin();
-        if (!ok) break;
-        uint32_t to = tmem + (g & (kSumsRing - 1)) * kN;
-        umma::mma_f16(to, da, db, id, !opens);
-        umma::mma_f16(to, umma::sdesc_at(da, 32), umma::sdesc_at(db, 32), id, 1);
-        if (parts == 2) {
-          umma::mma_commit(sums_full(g));
-          if (++g == groups) {
-            umma::mma_commit(freed(s));
-            break;
-          }
-          ok = begin();
-          if (!ok) break;
-          to = tmem + (g & (kSumsRing - 1)) * kN;
-        }
-        umma::mma_f16(to, umma::sdesc_at(da, 64), umma::sdesc_at(db, 64), id, parts == 1);
-        umma::mma_f16(to, umma::sdesc_at(da, 96), umma::sdesc_at(db, 96), id, 1);
-        if (closes) umma::mma_commit(sums_full(g++));
-        umma::mma_commit(freed(s));
+        to = acc0 + (g & (kSumsRing - 1)) * kN;
       }
-      if (!ok) {  // the MMAs issued so far end before their memory is given back
-        umma::mma_commit(drained);
-        umma::mbar_wait(drained, 0);
-      }
+      product(to, umma::sdesc_at(da, 64), umma::sdesc_at(db, 64), parts == 1);
+      product(to, umma::sdesc_at(da, 96), umma::sdesc_at(db, 96), 1);
+      if (closes) commit_if(leader, sums_full(g++));
+      commit_if(leader, freed(s));
     }
+    commit_if(leader, drained);  // the MMAs end, and their arrivals, before their memory is given back
+    umma::mbar_wait(drained, 0);
   } else {
     const int quarter = warp & 3, out = quarter * 32 + lane;
     const int64_t o = min(o0 + out, a.out_dim - 1);
@@ -495,19 +537,17 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(const __grid_c
       ok = __all_sync(0xffffffffu, umma::mbar_wait(sums_full(g), (uint32_t)(g / kSumsRing) & 1u));
       if (!ok) break;
       umma::fence_after();
+      const uint32_t from = tmem + (g & (kSumsRing - 1)) * kN + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll
       for (int n0 = 0; n0 < kN; n0 += 16) {
-        uint32_t r[16];
-        asm volatile(
-            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-              "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-            : "r"(tmem + (g & (kSumsRing - 1)) * kN + n0 + ((uint32_t)(quarter * 32) << 16)));
+        uint32_t r[16], u[16];
+        load16(from + n0, r);
+        if (kZeros) load16(from + kSumsRing * kN + n0, u);
         umma::tmem_wait_ld();
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float d = __uint_as_float(r[e]);
-          acc[n0 + e] = fmaf(s, kZeros ? fmaf(-z, x_sums[g * kN + n0 + e], d) : d, acc[n0 + e]);
+          acc[n0 + e] = fmaf(s, kZeros ? fmaf(-z, __uint_as_float(u[e]), d) : d, acc[n0 + e]);
         }
       }
       umma::fence_before();
@@ -586,19 +626,16 @@ bool encode(CUtensorMap* map, CUtensorMapDataType type, const m3_tensor& t, int6
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// (false: the sums of x of a very long row do not fit shared memory)
-template <typename T, int kN, bool kZeros> bool launch_many(const m3_w4_args& a, cudaStream_t stream, cudaError_t* e) {
+template <typename T, int kN, bool kZeros> cudaError_t launch_many(const m3_w4_args& a, cudaStream_t stream) {
   // CTAs for the columns of 128 outputs: while that leaves SMs idle and each has four slabs or more
   const int64_t tiles = (a.out_dim + kManyOuts - 1) / kManyOuts, slabs = (a.in_dim + kSlab - 1) / kSlab;
   const int64_t row_tiles = (a.rows + kN - 1) / kN;
   int split = 1;
   while (split < 8 && 2 * split * tiles * row_tiles <= sm_count() && slabs >= 8 * split) split *= 2;
-  const int64_t groups = (slabs + split - 1) / split * (kSlab / a.group);
-  const size_t smem = 1024 + std::max<size_t>(Many<kN>::kOffXSums + (kZeros ? groups * kN * 4 : 0), (size_t)kN * kManyOuts * 4);
-  if (smem > 227 * 1024) return false;
+  const size_t smem = Many<kN>::kBytes + (kZeros ? Many<kN>::kA : 0);
   auto kernel = w4_many_kernel<T, kN, kZeros>;
-  *e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (*e != cudaSuccess) return true;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = config(dim3((unsigned)(tiles * split), (unsigned)row_tiles), kManyThreads, smem, stream, attr);
   attr[1].id = cudaLaunchAttributeClusterDimension;
@@ -610,21 +647,18 @@ template <typename T, int kN, bool kZeros> bool launch_many(const m3_w4_args& a,
   const bool x_tiles = x_in_units(a) && a.x.stride[0] > 0;
   CUtensorMap code_map = {}, x_map = {};
   if ((code_tiles && !encode(&code_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, (a.in_dim + 1) / 2, a.out_dim, 1, kStage / 2,
-                             kManyOuts, CU_TENSOR_MAP_SWIZZLE_NONE)) ||
+                             kManyOuts, CU_TENSOR_MAP_SWIZZLE_32B)) ||
       (x_tiles && !encode(&x_map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                           a.x, a.in_dim, a.rows, 2, kStage, kN, CU_TENSOR_MAP_SWIZZLE_128B))) {
-    *e = cudaErrorInvalidValue;
-    return true;
+    return cudaErrorInvalidValue;
   }
-  *e = cudaLaunchKernelEx(&cfg, kernel, code_map, x_map, a, split, code_tiles, x_tiles);
-  return true;
+  return cudaLaunchKernelEx(&cfg, kernel, code_map, x_map, a, split, code_tiles, x_tiles);
 }
 
 // Past 64 rows, the weight is read once for every 64.
-template <typename T, bool kZeros> bool launch_many_rows(const m3_w4_args& a, cudaStream_t stream, cudaError_t* e) {
-  if (a.rows > 32 && launch_many<T, 64, kZeros>(a, stream, e)) return true;
-  if (a.rows > 16 && launch_many<T, 32, kZeros>(a, stream, e)) return true;
-  return launch_many<T, 16, kZeros>(a, stream, e);
+template <typename T, bool kZeros> cudaError_t launch_many_rows(const m3_w4_args& a, cudaStream_t stream) {
+  if (a.rows > 32) return launch_many<T, 64, kZeros>(a, stream);
+  return a.rows > 16 ? launch_many<T, 32, kZeros>(a, stream) : launch_many<T, 16, kZeros>(a, stream);
 }
 
 template <typename T, int kWords, bool kFast, bool kZeros> cudaError_t launch_few(const m3_w4_args& a, cudaStream_t stream) {
@@ -633,7 +667,7 @@ template <typename T, int kWords, bool kFast, bool kZeros> cudaError_t launch_fe
   int warps = 4;
   while (warps < kMostWarps && tiles * warps < (int64_t)16 * sm_count() && 4 * warps <= slabs) warps *= 2;
   cudaLaunchAttribute chained;
-  const cudaLaunchConfig_t cfg = config(dim3((unsigned)tiles, (unsigned)((a.rows + 7) / 8)), 32 * warps, 0, stream, &chained);
+  const cudaLaunchConfig_t cfg = config(dim3((unsigned)tiles), 32 * warps, 0, stream, &chained);
   return cudaLaunchKernelEx(&cfg, w4_few_kernel<T, kWords, kFast, kZeros>, a);
 }
 
@@ -647,8 +681,7 @@ template <typename T, int kWords> cudaError_t launch_group(const m3_w4_args& a, 
 }
 
 template <typename T> cudaError_t launch_type(const m3_w4_args& a, cudaStream_t stream) {
-  cudaError_t e = cudaSuccess;
-  if (a.rows > 8 && (a.zeros.data ? launch_many_rows<T, true>(a, stream, &e) : launch_many_rows<T, false>(a, stream, &e))) return e;
+  if (a.rows > 8) return a.zeros.data ? launch_many_rows<T, true>(a, stream) : launch_many_rows<T, false>(a, stream);
   switch (a.group) {
     case 32: return launch_group<T, 1>(a, stream);
     case 64: return launch_group<T, 2>(a, stream);
