@@ -9,6 +9,7 @@ namespace m3 {
 int read_device_error(int clear);
 int read_newton_error(int clear);
 int read_gated_error(int clear);
+int read_w4_error(int clear);
 
 cudaError_t launch_step(const m3_step_args& a, cudaStream_t stream);
 const char* last_step_kernel();
@@ -82,7 +83,8 @@ const char* m3_last_step_kernel(void) { return m3::last_step_kernel(); }
 int m3_device_error(int clear) {
   const int scan = m3::read_device_error(clear);  // synchronises the device
   const int newton = m3::read_newton_error(clear), gated = m3::read_gated_error(clear);
-  return scan != 0 ? scan : newton != 0 ? newton : gated;
+  const int w4 = m3::read_w4_error(clear);
+  return scan != 0 ? scan : newton != 0 ? newton : gated != 0 ? gated : w4;
 }
 
 int64_t m3_step_workspace_bytes(const m3_step_args* args) {
