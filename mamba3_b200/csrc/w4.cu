@@ -82,17 +82,18 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// kCount words of a row of codes from byte `at` on, any strides and alignment; bytes past the row are 0. Inside the row
-// they come as aligned words, shifted into place.
+// kCount words of a row of `bytes` bytes from byte `at` on, any alignment; bytes past the row are 0. Where they lie
+// inside the row, with what an aligned word more has, they come as aligned words, shifted into place.
 template <int kCount>
-__device__ __forceinline__ void row_words(const uint8_t* row, int64_t step, int at, int bytes, uint32_t* to) {
-  if (step == 1 && at >= 4 && at + 4 * kCount + 4 <= bytes) {
-    const uint8_t* from = row + at;
-    const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(from) & 3);
+__device__ __forceinline__ void row_words(const uint8_t* row, int64_t step, int64_t at, int64_t bytes, uint32_t* to) {
+  const uint8_t* from = row + at;
+  const int off = (int)(reinterpret_cast<uintptr_t>(from) & 3);
+  if (step == 1 && at >= off && at + 4 * kCount + (off ? 4 - off : 0) <= bytes) {
     const uint32_t* words = reinterpret_cast<const uint32_t*>(from - off);
     uint32_t held[kCount + 1];
 #pragma unroll
-    for (int i = 0; i <= kCount; ++i) held[i] = words[i];
+    for (int i = 0; i < kCount; ++i) held[i] = words[i];
+    held[kCount] = off ? words[kCount] : 0u;
 #pragma unroll
     for (int i = 0; i < kCount; ++i) to[i] = __funnelshift_r(held[i], held[i + 1], 8 * off);
   } else {
@@ -107,90 +108,114 @@ __device__ __forceinline__ void row_words(const uint8_t* row, int64_t step, int 
   }
 }
 
-// A value of a type known at run time, by its bits.
-__device__ __forceinline__ float widen(uint16_t v, bool bf16) {
-  return bf16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
+// A value of a type known at run time, by its bits. What is fetched ahead stays bits until it is used: a conversion would
+// wait for the load.
+__device__ __forceinline__ float widen(uint32_t v, int type) {
+  return type == M3_F32 ? __uint_as_float(v) : type == M3_BF16 ? __uint_as_float(v << 16) : __half2float(__ushort_as_half((uint16_t)v));
+}
+__device__ __forceinline__ uint32_t bits(const uint8_t* at, int type) {
+  return type == M3_F32 ? *reinterpret_cast<const uint32_t*>(at) : *reinterpret_cast<const uint16_t*>(at);
+}
+
+// Four bytes of a row from byte `at` on, which may lie before it or past it: 0 there.
+__device__ __noinline__ uint32_t edge_word(const uint8_t* row, int64_t step, int64_t at, int64_t bytes) {
+  uint32_t v = 0;
+  for (int b = 0; b < 4; ++b)
+    if (at + b >= 0 && at + b < bytes) v |= (uint32_t)row[(at + b) * step] << (8 * b);
+  return v;
 }
 
 // A warp's 16 output rows, as a thread sees them: rows g and g + 8 (past the end, the last one again: not written).
-// kFast: codes in whole aligned words, scales and zeros in 16 bits with unit stride along a row, columns a multiple of
-// 128: read without a check. Otherwise code by code.
+// kFast: codes in whole aligned words, scales and zeros in 16 bits with unit stride along a row, whole groups: read
+// group by group. Otherwise as aligned words around a row's own start, shifted into place where they are used, and byte
+// by byte at the tensor's ends or where a row's bytes lie apart.
 template <typename T, int kWords, bool kFast, bool kZeros> struct Weight {
-  static constexpr int kGroup = 32 * kWords, kPerSlab = kSlab / kGroup;
+  static constexpr int kGroup = 32 * kWords, kPerSlab = kSlab / kGroup, kHeld = kWords + (kFast ? 0 : 1);
   struct Slab {
-    uint32_t code[2][4];
-    float scale[2][kPerSlab], shift[2][kZeros ? kPerSlab : 1];  // s and z - 8 of the slab's groups
+    uint32_t code[2][kPerSlab][kHeld];
+    uint32_t scale[2][kPerSlab], zero[2][kZeros ? kPerSlab : 1];  // bits
   };
   const m3_w4_args& a;
-  const uint8_t* code[2];
-  const uint16_t *scale[2], *zero[2];
-  int64_t row[2];
-  int t, in_dim, slabs;
+  const uint8_t *code[2], *scale[2], *zero[2];
+  int t, in_dim, slabs, type, size;
+  int off[2];
 
   __device__ __forceinline__ Weight(const m3_w4_args& args, int64_t o0, int lane) : a(args), t(lane & 3), in_dim((int)args.in_dim) {
     slabs = (in_dim + kSlab - 1) / kSlab;
+    type = a.scales.dtype;
+    size = !kFast && type == M3_F32 ? 4 : 2;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      row[r] = min(o0 + (lane >> 2) + 8 * r, a.out_dim - 1);
-      code[r] = static_cast<const uint8_t*>(a.codes.data) + row[r] * a.codes.stride[0] + (kFast ? 4 * kWords * t : 0);
-      if constexpr (kFast) {
-        scale[r] = static_cast<const uint16_t*>(a.scales.data) + row[r] * a.scales.stride[0];
-        if (kZeros) zero[r] = static_cast<const uint16_t*>(a.zeros.data) + row[r] * a.zeros.stride[0];
-      }
+      const int64_t row = min(o0 + (lane >> 2) + 8 * r, a.out_dim - 1);
+      code[r] = static_cast<const uint8_t*>(a.codes.data) + row * a.codes.stride[0] + (kFast ? 4 * kWords * t : 0);
+      off[r] = !kFast && a.codes.stride[1] == 1 ? (int)(reinterpret_cast<uintptr_t>(code[r]) & 3) : 0;
+      scale[r] = static_cast<const uint8_t*>(a.scales.data) + row * a.scales.stride[0] * size;
+      if (kZeros) zero[r] = static_cast<const uint8_t*>(a.zeros.data) + row * a.zeros.stride[0] * size;
     }
   }
+  // A slab's first column: of whole groups that leave the last slab short, that one is the row's last 128 columns, less the
+  // groups that the slab before had.
+  __device__ __forceinline__ int from(int slab) const { return kFast && kPerSlab > 1 ? min(slab * kSlab, in_dim - kSlab) : slab * kSlab; }
   // Pull a slab's codes towards L2.
   __device__ __forceinline__ void prefetch(int slab) const {
     if (kFast && slab < slabs)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) asm volatile("prefetch.global.L2 [%0];" ::"l"(code[r] + slab * (kSlab / 2)));
+      for (int r = 0; r < 2; ++r) asm volatile("prefetch.global.L2 [%0];" ::"l"(code[r] + from(slab) / 2));
   }
   __device__ __forceinline__ void fetch(int slab, Slab& to) const {
     if (slab >= slabs) return;
+    const int begin = from(slab);
     if constexpr (kFast) {
-      const bool bf16 = a.scales.dtype == M3_BF16;
 #pragma unroll
       for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int c = 0; c < kPerSlab; ++c) {
-          const uint8_t* from = code[r] + slab * (kSlab / 2) + c * (kGroup / 2);
+          const uint8_t* at = code[r] + begin / 2 + c * (kGroup / 2);
           if constexpr (kWords == 1) {
-            to.code[r][c] = __ldcs(reinterpret_cast<const unsigned int*>(from));
+            to.code[r][c][0] = __ldcs(reinterpret_cast<const unsigned int*>(at));
           } else if constexpr (kWords == 2) {
-            const uint2 v = __ldcs(reinterpret_cast<const uint2*>(from));
-            to.code[r][2 * c] = v.x;
-            to.code[r][2 * c + 1] = v.y;
+            const uint2 v = __ldcs(reinterpret_cast<const uint2*>(at));
+            to.code[r][c][0] = v.x;
+            to.code[r][c][1] = v.y;
           } else {
-            const uint4 v = __ldcs(reinterpret_cast<const uint4*>(from));
-            to.code[r][0] = v.x;
-            to.code[r][1] = v.y;
-            to.code[r][2] = v.z;
-            to.code[r][3] = v.w;
+            const uint4 v = __ldcs(reinterpret_cast<const uint4*>(at));
+            to.code[r][c][0] = v.x;
+            to.code[r][c][1] = v.y;
+            to.code[r][c][2] = v.z;
+            to.code[r][c][3] = v.w;
           }
-          to.scale[r][c] = widen(scale[r][slab * kPerSlab + c], bf16);
-          if (kZeros) to.shift[r][c] = widen(zero[r][slab * kPerSlab + c], bf16) - 8.0f;
+          to.scale[r][c] = *reinterpret_cast<const uint16_t*>(scale[r] + 2 * (begin / kGroup + c));
+          if (kZeros) to.zero[r][c] = *reinterpret_cast<const uint16_t*>(zero[r] + 2 * (begin / kGroup + c));
         }
     } else {
-      careful(slab, to);
-    }
-  }
-  // Any strides, and the end of a row: bytes past it are 0 (x is 0 there), and so are scales.
-  __device__ __forceinline__ void careful(int slab, Slab& to) const {
-    const int bytes = (in_dim + 1) / 2;
+      const int bytes = (in_dim + 1) / 2;
+      const uint8_t* data = static_cast<const uint8_t*>(a.codes.data);
+      const uint8_t* end = data + (a.out_dim - 1) * a.codes.stride[0] + bytes;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const uint8_t* from = static_cast<const uint8_t*>(a.codes.data) + row[r] * a.codes.stride[0];
+      for (int r = 0; r < 2; ++r) {
+        // a neighbour row's bytes do no harm: they are shifted out, or meet zeros of x
+        const bool inside = a.codes.stride[1] == 1 && a.codes.stride[0] >= 0 && code[r] + begin / 2 - off[r] >= data &&
+                            code[r] + begin / 2 + kSlab / 2 + 4 <= end;
 #pragma unroll
-      for (int c = 0; c < kPerSlab; ++c)
-        row_words<kWords>(from, a.codes.stride[1], slab * (kSlab / 2) + c * (kGroup / 2) + 4 * kWords * t, bytes, to.code[r] + c * kWords);
+        for (int c = 0; c < kPerSlab; ++c) {
+          const int at = begin / 2 + c * (kGroup / 2) + 4 * kWords * t - off[r];
+          const int group = begin / kGroup + c;
+          const bool there = group * kGroup < in_dim;  // past the row, x is 0
+          if (inside) {
 #pragma unroll
-      for (int c = 0; c < kPerSlab; ++c) {
-        const int group = slab * kPerSlab + c;
-        const bool there = group * kGroup < in_dim;
-        to.scale[r][c] = there ? ld_t(a.scales, row[r] * a.scales.stride[0] + group * a.scales.stride[1]) : 0.0f;
-        if (kZeros) to.shift[r][c] = there ? ld_t(a.zeros, row[r] * a.zeros.stride[0] + group * a.zeros.stride[1]) - 8.0f : 0.0f;
+            for (int w = 0; w <= kWords; ++w) to.code[r][c][w] = *reinterpret_cast<const uint32_t*>(code[r] + at + 4 * w);
+          } else {
+#pragma unroll
+            for (int w = 0; w <= kWords; ++w) to.code[r][c][w] = edge_word(code[r], a.codes.stride[1], at + 4 * w, bytes);
+          }
+          to.scale[r][c] = there ? bits(scale[r] + group * a.scales.stride[1] * size, type) : 0u;
+          if (kZeros) to.zero[r][c] = there ? bits(zero[r] + group * a.zeros.stride[1] * size, type) : 0u;
+        }
       }
     }
+  }
+  __device__ __forceinline__ uint32_t word(const Slab& s, int r, int c, int w) const {
+    return kFast ? s.code[r][c][w] : __funnelshift_r(s.code[r][c][w], s.code[r][c][kFast ? w : w + 1], 8 * off[r]);
   }
 };
 
@@ -204,17 +229,17 @@ __device__ __forceinline__ void join(float (&acc)[4], const float (&d)[4], const
   acc[3] = fmaf(s1, kZeros ? fmaf(-z1, sums[1], d[3]) : d[3], acc[3]);
 }
 
-// 8 columns of a row of x, from column c on; 0 past the row.
+// 8 columns of a row of x, from column c on; 0 past the row. `units`: rows start on 16 bytes.
 template <typename T> __device__ __noinline__ uint4 x_careful(const m3_w4_args& a, const T* row, int c) {
   uint32_t w[4] = {0, 0, 0, 0};
-  if (a.x.stride[1] == 1 && c + 8 <= a.in_dim) {
+  if (a.x.stride[1] == 1) {
+    row_words<4>(reinterpret_cast<const uint8_t*>(row), 1, 2 * (int64_t)c, 2 * a.in_dim, w);
+  } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[c + e] << (16 * (e & 1));
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    for (int e = 0; e < 8; ++e)
+      if (c + e < a.in_dim)
+        w[e >> 1] |= (uint32_t)*reinterpret_cast<const uint16_t*>(row + (c + e) * a.x.stride[1]) << (16 * (e & 1));
   }
-  for (int e = 0; e < 8; ++e)
-    if (c + e < a.in_dim)
-      w[e >> 1] |= (uint32_t)*reinterpret_cast<const uint16_t*>(row + (c + e) * a.x.stride[1]) << (16 * (e & 1));
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 template <typename T> __device__ __forceinline__ uint4 x_unit(const m3_w4_args& a, const T* row, int c, bool units) {
@@ -243,8 +268,10 @@ __global__ void __launch_bounds__(32 * kMostWarps) w4_few_kernel(const m3_w4_arg
   // the wait. Until then the first codes are pulled towards L2.
   for (int i = 0; i < kAhead; ++i) weight.prefetch(warp + i * warps);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const bool units = x_in_units(a), here = g < a.rows;
-  const T* row = static_cast<const T*>(a.x.data) + (here ? g : 0) * a.x.stride[0];
+  const bool units = x_in_units(a);
+  // (a thread's type of scales: 16 bits in the fast form)
+  auto value = [&](uint32_t v) { return kFast ? (weight.type == M3_BF16 ? __uint_as_float(v << 16) : __half2float(__ushort_as_half((uint16_t)v))) : widen(v, weight.type); };
+  const T* row = static_cast<const T*>(a.x.data) + min(g, (int)a.rows - 1) * a.x.stride[0];  // past the last row: the last, not written
   typename W::Slab held[kAhead];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) weight.fetch(warp + i * warps, held[i]);
@@ -256,24 +283,37 @@ __global__ void __launch_bounds__(32 * kMostWarps) w4_few_kernel(const m3_w4_arg
       const int slab = slab0 + i * warps;
       if (slab >= weight.slabs) break;
       uint4 x[4];
+      const int begin = weight.from(slab);
+      const T* columns = row + begin + 8 * kWords * t;  // of word w: group w / kWords of the slab
+      if (kFast) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {  // columns of word w of a thread: group w / kWords of the slab
-        const int c = slab * kSlab + w / kWords * W::kGroup + 8 * (kWords * t + w % kWords);
-        x[w] = make_uint4(0u, 0u, 0u, 0u);
-        if constexpr (kFast) {
-          if (here) x[w] = *reinterpret_cast<const uint4*>(row + c);
-        } else {
-          if (here) x[w] = x_unit(a, row, c, units);
+        for (int w = 0; w < 4; ++w) x[w] = *reinterpret_cast<const uint4*>(columns + w / kWords * W::kGroup + 8 * (w % kWords));
+      } else if (a.x.stride[1] == 1 && begin >= 2 && begin + kSlab + 2 <= weight.in_dim) {
+        const int off = (int)(reinterpret_cast<uintptr_t>(columns) & 3);
+        uint32_t v[4][5];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint8_t* at = reinterpret_cast<const uint8_t*>(columns + w / kWords * W::kGroup + 8 * (w % kWords)) - off;
+#pragma unroll
+          for (int e = 0; e < 5; ++e) v[w][e] = reinterpret_cast<const uint32_t*>(at)[e];
         }
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          x[w] = make_uint4(__funnelshift_r(v[w][0], v[w][1], 8 * off), __funnelshift_r(v[w][1], v[w][2], 8 * off),
+                            __funnelshift_r(v[w][2], v[w][3], 8 * off), __funnelshift_r(v[w][3], v[w][4], 8 * off));
+      } else {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) x[w] = x_unit(a, row, begin + w / kWords * W::kGroup + 8 * (kWords * t + w % kWords), units);
       }
 #pragma unroll
       for (int c = 0; c < W::kPerSlab; ++c) {
+        if (kFast && W::kPerSlab > 1 && begin + c * W::kGroup < slab * kSlab) continue;  // the slab before had it
         float d[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int w = 0; w < kWords; ++w) {
           uint32_t low[4], high[4];
-          open8<T>(held[i].code[0][c * kWords + w], low);
-          open8<T>(held[i].code[1][c * kWords + w], high);
+          open8<T>(weight.word(held[i], 0, c, w), low);
+          open8<T>(weight.word(held[i], 1, c, w), high);
           const uint4 b = x[c * kWords + w];
           mma<T>(d, low[0], high[0], low[1], high[1], b.x, b.y);
           mma<T>(d, low[2], high[2], low[3], high[3], b.z, b.w);
@@ -282,8 +322,9 @@ __global__ void __launch_bounds__(32 * kMostWarps) w4_few_kernel(const m3_w4_arg
             mma<T>(sums, one2, one2, one2, one2, b.z, b.w);
           }
         }
-        join<kZeros>(acc, d, sums, held[i].scale[0][c], held[i].scale[1][c], held[i].shift[0][kZeros ? c : 0],
-                     held[i].shift[1][kZeros ? c : 0]);
+        constexpr int kZ = kZeros ? 1 : 0;
+        join<kZeros>(acc, d, sums, value(held[i].scale[0][c]), value(held[i].scale[1][c]), value(held[i].zero[0][kZ * c]) - 8.0f,
+                     value(held[i].zero[1][kZ * c]) - 8.0f);
       }
       weight.fetch(slab + kAhead * warps, held[i]);
     }
@@ -317,10 +358,12 @@ __global__ void __launch_bounds__(32 * kMostWarps) w4_few_kernel(const m3_w4_arg
 // vector registers, took 24 at 64 rows; stages of 128 columns 19.5; the warp-level instruction 15.3, 19.8 and 31.
 constexpr int kManyOuts = 128, kStage = 64;  // outputs of a CTA, columns of a stage
 constexpr int kStages = 4, kRing = 8;        // of codes as 16-bit values; of codes and x as they come (powers of two)
-constexpr int kTeams = 3, kProducers = 128 * kTeams, kManyThreads = kProducers + 64 + 128;
+constexpr int kTeams = 3, kProducers = 128 * kTeams;
 constexpr int kSumsRing = 4;
 
 template <int kN> struct Many {
+  static constexpr int kCols = kN < 32 ? kN : 32, kConsumers = 4 * (kN / kCols);  // columns of a thread's sums; warps
+  static constexpr int kThreads = kProducers + 64 + 32 * kConsumers;
   static constexpr uint32_t kA = kManyOuts * kStage * 2, kX = kN * kStage * 2, kCodes = kManyOuts * kStage / 2;
   static constexpr uint32_t kOffX = kStages * kA, kOffCodes = kOffX + kRing * kX, kOffBars = kOffCodes + kRing * kCodes;
   static constexpr uint32_t kOffOnes = kOffBars + 1024;  // a tile of ones, with zero points only
@@ -346,7 +389,13 @@ __device__ __forceinline__ void commit_if(uint32_t leader, uint32_t bar) {
       : "memory");
 }
 
-__device__ __forceinline__ void load16(uint32_t from, uint32_t (&r)[16]) {
+// Columns of tensor memory from `from` on, this thread's row of them.
+__device__ __forceinline__ void load(uint32_t from, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(from));
+}
+__device__ __forceinline__ void load(uint32_t from, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
@@ -355,7 +404,7 @@ __device__ __forceinline__ void load16(uint32_t from, uint32_t (&r)[16]) {
 }
 
 template <typename T, int kN, bool kZeros>
-__global__ void __launch_bounds__(kManyThreads, 1)
+__global__ void __launch_bounds__(Many<kN>::kThreads, 1)
     w4_many_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_constant__ CUtensorMap x_map, const m3_w4_args a,
                    int split, bool code_tiles, bool x_tiles) {
   using M = Many<kN>;
@@ -392,7 +441,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     }
     for (int i = 0; i < kSumsRing; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(sums_full(i)));
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 4;" ::"r"(sums_empty(i)));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(sums_empty(i)), "r"(M::kConsumers));
     }
     asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(drained));
     asm volatile("fence.mbarrier_init.release.cluster;");
@@ -408,7 +457,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   const T* xp = static_cast<const T*>(a.x.data) + rows0 * a.x.stride[0];
   if (kZeros) {
     const uint32_t one2 = std::is_same<T, __half>::value ? 0x3C003C00u : 0x3F803F80u;
-    for (int i = tid; i < (int)M::kA / 16; i += kManyThreads)
+    for (int i = tid; i < (int)M::kA / 16; i += M::kThreads)
       asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(base + M::kOffOnes + 16 * i), "r"(one2) : "memory");
     umma::fence_async_smem();
   }
@@ -417,16 +466,67 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   umma::fence_after();
   uint32_t tmem;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
-  float acc[kN];  // the consumers' sums
+  float acc[M::kCols];  // the consumers' sums
 
   if (tid < kProducers) {
     // the teams take stages in turn; a thread's part of one is the 64 columns of an output
-    const int out = tid & 127, flip = (out >> 2) & 1;  // (the copy's 32-byte swizzle: halves change places every four rows)
-    const uint8_t* codes = static_cast<const uint8_t*>(a.codes.data) + min(o0 + out, a.out_dim - 1) * a.codes.stride[0];
+    const int out = tid & 127, team = warp >> 2, flip = (out >> 2) & 1;  // (the copy's 32-byte swizzle: halves change places every four rows)
+    const uint8_t* data = static_cast<const uint8_t*>(a.codes.data);
+    const uint8_t* codes = data + min(o0 + out, a.out_dim - 1) * a.codes.stride[0];
+    const int bytes = (in_dim + 1) / 2;
+    // Rows of bytes that no copy engine reads (not a multiple of 16 bytes apart) come as aligned words, nine a row and
+    // stage, the team's threads along the rows, a turn ahead in registers; shared memory hands each thread its row.
+    const bool staged = !code_tiles && a.codes.stride[1] == 1 && a.codes.stride[0] >= 0;
+    const uint8_t* end = data + (a.out_dim - 1) * a.codes.stride[0] + bytes;
+    const uint32_t staging = base + M::kOffCodes + team * (kManyOuts * 36);
+    uint32_t ahead[9];
+    auto fetch_rows = [&](int s) {
+#pragma unroll
+      for (int j = 0; j < 9; ++j) {
+        const int i = 128 * j + out;
+        const uint8_t* from = data + min(o0 + i / 9, a.out_dim - 1) * a.codes.stride[0] + (first + s * kStage) / 2;
+        from += 4 * (i % 9) - (int)(reinterpret_cast<uintptr_t>(from) & 3);
+        if (from >= data && from + 4 <= end) {
+          ahead[j] = *reinterpret_cast<const uint32_t*>(from);
+        } else {
+          uint32_t v = 0;
+          for (int b = 0; b < 4; ++b)
+            if (from + b >= data && from + b < end) v |= (uint32_t)from[b] << (8 * b);
+          ahead[j] = v;
+        }
+      }
+    };
+    if (staged && team < stages) fetch_rows(team);
     bool ok = true;
-    for (int s = tid >> 7; s < stages; s += kTeams) {
+    for (int s = team; s < stages; s += kTeams) {
       uint32_t words[8];
-      if (!code_tiles) row_words<8>(codes, a.codes.stride[1], (first + s * kStage) / 2, (in_dim + 1) / 2, words);
+      uint4 held[kN / 16];
+      const int c0 = first + s * kStage;
+      if (!x_tiles) {
+        if (a.x.stride[1] == 1 && c0 >= 2 && c0 + kStage + 2 <= in_dim) {  // rows past the last: the last, not written
+          uint32_t w[kN / 16][5];
+          int off[kN / 16];
+#pragma unroll
+          for (int i = 0; i < kN / 16; ++i) {
+            const T* from = xp + min((out >> 3) + 16 * i, rows - 1) * a.x.stride[0] + c0 + 8 * (out & 7);
+            off[i] = (int)(reinterpret_cast<uintptr_t>(from) & 3);
+            const uint32_t* aligned = reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(from) - off[i]);
+#pragma unroll
+            for (int e = 0; e < 5; ++e) w[i][e] = aligned[e];
+          }
+#pragma unroll
+          for (int i = 0; i < kN / 16; ++i)
+            held[i] = make_uint4(__funnelshift_r(w[i][0], w[i][1], 8 * off[i]), __funnelshift_r(w[i][1], w[i][2], 8 * off[i]),
+                                 __funnelshift_r(w[i][2], w[i][3], 8 * off[i]), __funnelshift_r(w[i][3], w[i][4], 8 * off[i]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < kN / 16; ++i) {
+            const int n = (out >> 3) + 16 * i, c = c0 + 8 * (out & 7);
+            held[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (n < rows && c < in_dim) held[i] = x_unit(a, xp + n * a.x.stride[0], c, units);
+          }
+        }
+      }
       if (ok) ok = umma::mbar_wait(came(s), (uint32_t)(s / kRing) & 1u);
       if (code_tiles) {
         const uint32_t from = base + M::kOffCodes + (s & (kRing - 1)) * M::kCodes + out * 32;
@@ -436,15 +536,30 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                        : "=r"(words[4 * h]), "=r"(words[4 * h + 1]), "=r"(words[4 * h + 2]), "=r"(words[4 * h + 3])
                        : "r"(from + ((h ^ flip) << 4))
                        : "memory");
+      } else if (staged) {
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + team) : "memory");  // the team has read what this one replaces
+#pragma unroll
+        for (int j = 0; j < 9; ++j) asm volatile("st.shared.u32 [%0], %1;" ::"r"(staging + 4 * (128 * j + out)), "r"(ahead[j]) : "memory");
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + team) : "memory");
+        if (s + kTeams < stages) fetch_rows(s + kTeams);
+        const int off = (int)(reinterpret_cast<uintptr_t>(codes + c0 / 2) & 3);
+        uint32_t w[9];
+#pragma unroll
+        for (int j = 0; j < 9; ++j) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[j]) : "r"(staging + 36 * out + 4 * j) : "memory");
+#pragma unroll
+        for (int j = 0; j < 8; ++j) words[j] = __funnelshift_r(w[j], w[j + 1], 8 * off);
+      } else {
+        row_words<8>(codes, a.codes.stride[1], c0 / 2, bytes, words);
       }
       // the MMAs of stage s - kStages are done with what this one replaces
       if (s >= kStages && ok) ok = umma::mbar_wait(freed(s - kStages), (uint32_t)((s - kStages) / kRing) & 1u);
       if (!x_tiles)
-        for (int i = out; i < kN * (kStage / 8); i += 128) {
-          const int n = i >> 3, u = i & 7, c = first + s * kStage + 8 * u;
-          const uint4 v = n < rows && c < in_dim ? x_unit(a, xp + n * a.x.stride[0], c, units) : make_uint4(0u, 0u, 0u, 0u);
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(base + M::kOffX + (s & (kRing - 1)) * M::kX + n * 128 + ((u ^ (n & 7)) << 4)),
-                       "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+#pragma unroll
+        for (int i = 0; i < kN / 16; ++i) {
+          const int n = (out >> 3) + 16 * i;
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(base + M::kOffX + (s & (kRing - 1)) * M::kX + n * 128 +
+                                                                        (((out ^ n) & 7) << 4)),
+                       "r"(held[i].x), "r"(held[i].y), "r"(held[i].z), "r"(held[i].w)
                        : "memory");
         }
       const uint32_t to = base + (s & (kStages - 1)) * M::kA + out * 128;
@@ -539,30 +654,50 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     commit_if(leader, drained);  // the MMAs end, and their arrivals, before their memory is given back
     umma::mbar_wait(drained, 0);
   } else {
-    const int quarter = warp & 3, out = quarter * 32 + lane;
+    const int quarter = warp & 3, out = quarter * 32 + lane, col0 = M::kCols * ((warp - kProducers / 32 - 2) >> 2);
     const int64_t o = min(o0 + out, a.out_dim - 1);
-    const int64_t scale_at = o * a.scales.stride[0], zero_at = o * a.zeros.stride[0];
 #pragma unroll
-    for (int n = 0; n < kN; ++n) acc[n] = 0.0f;
-    auto value = [&](const m3_tensor& t, int64_t at, int g) { return g < groups ? ld_t(t, at + (first / a.group + g) * t.stride[1]) : 0.0f; };
-    float s_next = value(a.scales, scale_at, 0), z_next = kZeros ? value(a.zeros, zero_at, 0) : 0.0f;
+    for (int n = 0; n < M::kCols; ++n) acc[n] = 0.0f;
+    const int type = a.scales.dtype, size = type == M3_F32 ? 4 : 2;
+    auto start = [&](const m3_tensor& t) {
+      return static_cast<const uint8_t*>(t.data) + (o * t.stride[0] + first / a.group * t.stride[1]) * size;
+    };
+    auto fetch = [&](const uint8_t*& at, int64_t stride, int g) {
+      const uint32_t v = g < groups ? bits(at, type) : 0u;
+      at += stride * size;
+      return v;
+    };
+    auto value = [&](uint32_t v) { return widen(v, type); };
+    const uint8_t *scale_at = start(a.scales), *zero_at = kZeros ? start(a.zeros) : nullptr;
+    constexpr int kPart = kZeros ? 8 : 16;  // columns read at a time
+    constexpr int kAhead = kZeros ? 2 : 4;  // groups whose scales are under way
+    uint32_t s_held[kAhead], z_held[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      s_held[i] = fetch(scale_at, a.scales.stride[1], i);
+      z_held[i] = kZeros ? fetch(zero_at, a.zeros.stride[1], i) : 0u;
+    }
     bool ok = true;
-    for (int g = 0; g < groups; ++g) {
-      const float s = s_next, z = z_next - 8.0f;
-      s_next = value(a.scales, scale_at, g + 1);
-      if (kZeros) z_next = value(a.zeros, zero_at, g + 1);
+    for (int g0 = 0; g0 < groups && ok; g0 += kAhead)
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int g = g0 + i;
+      if (g >= groups) break;
+      const float s = value(s_held[i]), z = value(z_held[i]) - 8.0f;
+      s_held[i] = fetch(scale_at, a.scales.stride[1], g + kAhead);
+      if (kZeros) z_held[i] = fetch(zero_at, a.zeros.stride[1], g + kAhead);
       ok = __all_sync(0xffffffffu, umma::mbar_wait(sums_full(g), (uint32_t)(g / kSumsRing) & 1u));
       if (!ok) break;
       umma::fence_after();
-      const uint32_t from = tmem + (g & (kSumsRing - 1)) * kN + ((uint32_t)(quarter * 32) << 16);
+      const uint32_t from = tmem + (g & (kSumsRing - 1)) * kN + col0 + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll
-      for (int n0 = 0; n0 < kN; n0 += 16) {
-        uint32_t r[16], u[16];
-        load16(from + n0, r);
-        if (kZeros) load16(from + kSumsRing * kN + n0, u);
+      for (int n0 = 0; n0 < M::kCols; n0 += kPart) {
+        uint32_t r[kPart], u[kPart];
+        load(from + n0, r);
+        if (kZeros) load(from + kSumsRing * kN + n0, u);
         umma::tmem_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int e = 0; e < kPart; ++e) {
           const float d = __uint_as_float(r[e]);
           acc[n0 + e] = fmaf(s, kZeros ? fmaf(-z, __uint_as_float(u[e]), d) : d, acc[n0 + e]);
         }
@@ -581,11 +716,12 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   T* yp = static_cast<T*>(a.y.data);
   const int out = (warp & 3) * 32 + lane;
   const bool consumer = warp > kProducers / 32 + 1;
+  const int col0 = consumer ? M::kCols * ((warp - kProducers / 32 - 2) >> 2) : 0;
   if (split == 1) {
     if (consumer && o0 + out < a.out_dim) {
 #pragma unroll
-      for (int n = 0; n < kN; ++n)
-        if (n < rows) yp[(rows0 + n) * a.y.stride[0] + (o0 + out) * a.y.stride[1]] = from_f<T>(acc[n]);
+      for (int n = 0; n < M::kCols; ++n)
+        if (col0 + n < rows) yp[(rows0 + col0 + n) * a.y.stride[0] + (o0 + out) * a.y.stride[1]] = from_f<T>(acc[n]);
     }
     return;
   }
@@ -593,13 +729,13 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   float* part = reinterpret_cast<float*>(smem);
   if (consumer) {
 #pragma unroll
-    for (int n = 0; n < kN; ++n) part[n * kManyOuts + out] = acc[n];
+    for (int n = 0; n < M::kCols; ++n) part[(col0 + n) * kManyOuts + out] = acc[n];
   }
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   const int share = kN / split;
-  for (int i = tid; i < share * kManyOuts; i += kManyThreads) {
+  for (int i = tid; i < share * kManyOuts; i += M::kThreads) {
     const int n = rank * share + i / kManyOuts, oo = i % kManyOuts;
     float v = 0.0f;
     for (int r = 0; r < split; ++r) {
@@ -654,7 +790,7 @@ template <typename T, int kN, bool kZeros> cudaError_t launch_many(const m3_w4_a
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[2];
-  cudaLaunchConfig_t cfg = config(dim3((unsigned)(tiles * split), (unsigned)row_tiles), kManyThreads, smem, stream, attr);
+  cudaLaunchConfig_t cfg = config(dim3((unsigned)(tiles * split), (unsigned)row_tiles), Many<kN>::kThreads, smem, stream, attr);
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = split;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
@@ -691,8 +827,7 @@ template <typename T, int kWords, bool kFast, bool kZeros> cudaError_t launch_fe
 template <typename T, int kWords> cudaError_t launch_group(const m3_w4_args& a, cudaStream_t stream) {
   const bool fast = a.codes.stride[1] == 1 && a.codes.stride[0] % (4 * kWords) == 0 &&
                     reinterpret_cast<uintptr_t>(a.codes.data) % (4 * kWords) == 0 && a.scales.dtype != M3_F32 && x_in_units(a) &&
-                    a.in_dim % kSlab == 0 &&
-                    a.scales.stride[1] == 1 && (a.zeros.data == nullptr || a.zeros.stride[1] == 1);
+                    a.in_dim % a.group == 0 && a.in_dim >= kSlab && a.scales.stride[1] == 1 && (a.zeros.data == nullptr || a.zeros.stride[1] == 1);
   if (a.zeros.data) return fast ? launch_few<T, kWords, true, true>(a, stream) : launch_few<T, kWords, false, true>(a, stream);
   return fast ? launch_few<T, kWords, true, false>(a, stream) : launch_few<T, kWords, false, false>(a, stream);
 }
