@@ -69,7 +69,7 @@ def test_model_sizes_and_float32_scales(shape):
 
 
 def test_very_long_rows():
-    """More groups than the many-row kernel has shared memory for the sums of x."""
+    """Thousands of groups with zero points, more than any table of them in shared memory would hold."""
     codes, scales, zero = _weight(20, 120000, 32, True, torch.float16)
     x = torch.randn(18, 120000, device="cuda").to(torch.float16)
     _check(x, codes, scales, zero, 32, linear_w4(x, codes, scales, zero, group_size=32))
@@ -84,6 +84,31 @@ def test_strides_and_offsets():
         for q in (codes, wide_codes[:, 3:131], codes.t().contiguous().t()):
             for s in (scales, scales.t().contiguous().t()):
                 _check(x, q, s, zero, 32, linear_w4(x, q, s, zero, group_size=32))
+
+
+@pytest.mark.parametrize("rows", [1, 8, 12, 40])
+@pytest.mark.parametrize("in_dim,group", [(160, 32), (192, 64), (1120, 32), (2624, 64), (96, 32)])
+def test_whole_groups_that_leave_a_short_end(rows, in_dim, group):
+    codes, scales, zero = _weight(77, in_dim, group, rows % 8 == 0, torch.bfloat16)
+    x = torch.randn(rows, in_dim, device="cuda").to(torch.bfloat16)
+    _check(x, codes, scales, zero, group, linear_w4(x, codes, scales, zero, group_size=group))
+
+
+@pytest.mark.parametrize("rows", [1, 3, 20, 64])
+@pytest.mark.parametrize("offset", [0, 1, 2, 3])
+def test_unaligned_rows_between_other_values(rows, offset):
+    """Rows of codes and of x that start anywhere, with NaN around x and other bytes around the codes."""
+    out_dim, in_dim = 131, 1283
+    codes, scales, zero = _weight(out_dim, in_dim, 32, offset % 2 == 1, torch.float16, seed=offset)
+    scales, zero = scales.float(), None if zero is None else zero.float()
+    bytes_ = codes.shape[1]
+    flat = torch.full((offset + out_dim * bytes_,), 255, device="cuda", dtype=torch.uint8)
+    packed = flat[offset:].view(out_dim, bytes_)
+    packed.copy_(codes)
+    wide = torch.full((rows, in_dim + 9), torch.nan, device="cuda", dtype=torch.float16)
+    x = wide[:, offset:offset + in_dim]
+    x.copy_(torch.randn(rows, in_dim, device="cuda"))
+    _check(x, packed, scales, zero, 32, linear_w4(x, packed, scales, zero, group_size=32))
 
 
 def test_zero_scales_and_nonfinite_rows():
