@@ -679,14 +679,16 @@ cudaError_t launch_tiles(K kernel, const m3_gated_args& a, const Maps& maps, int
   const int64_t blocks = (int64_t)a.batch * ((a.channels + kChannels - 1) / kChannels);
   // A cluster takes a sequence's tiles together while its CTAs still have room on the GPU at once: clusters of up to
   // 4 in all the room there is (4 x 2048 x 2048: 47 us in fours, 54 in twos), larger ones, whose exchange takes as long
-  // as a tile, up to two CTAs an SM (1 x 65536 x 1536: 317 us in eights, 339 in sixteens; 1 x 32768 x 128: 83 us in
-  // sixteens, 136 in eights). Past 8 CTAs, a cluster's size without conditions, only where two fit an SM.
+  // as a tile, up to two CTAs an SM (1 x 65536 x 1536: 308 us in eights, 328 in sixteens; 1 x 32768 x 128: 83 us in
+  // sixteens, 136 in eights), and tens where sixteens have no such room (1 x 65536 x 1536: 267 us, backward 647 against
+  // 762). Past 8 CTAs, a cluster's size without conditions, only where two fit an SM.
   const int per_sm = 227 * 1024 / (smem_bytes(tile, tensors, run_maps, 2) + 1024);
   const int most = per_sm > 1 ? kMaxCluster : 8;
   int cluster = 1;
   while (cluster < most && 2 * cluster <= ntiles &&
          2 * cluster * blocks <= (int64_t)sm_count() * (cluster < 4 ? per_sm : std::min(per_sm, 2)))
     cluster *= 2;
+  if (cluster == 8 && most > 8 && 10 <= ntiles && 10 * blocks <= 2 * (int64_t)sm_count()) cluster = 10;
   const int smem = smem_bytes(tile, tensors, run_maps, cluster);
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;

@@ -119,6 +119,25 @@ def test_backward_many_tiles_and_strided_dy():
         assert_rounded(a, e, 2 * SUMS)
 
 
+@pytest.mark.parametrize("length", [650, 1300])
+@pytest.mark.parametrize("channels", [128, 1216, 1300, 2368, 4736, 9600])
+def test_every_split_of_a_sequence(length, channels):
+    """1 to 16 CTAs walk a sequence's tiles together, by how many channels there are."""
+    value, forget, gate, state, reset = _inputs(1, length, channels, torch.bfloat16, seed=channels)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    dy = torch.randn(1, length, channels, device="cuda", generator=g).to(torch.bfloat16)
+    dstate = torch.randn(1, channels, device="cuda", generator=g)
+    run = lambda v, f, q, s, r: gated_scan(v, f, q, initial_state=s, reset=r)  # noqa: E731
+    y, final = run(value, forget, gate, state, reset)
+    want_y, want_final = gated_scan64(value, forget, gate, state, reset)
+    assert_rounded(y, want_y, SUMS)
+    assert_rounded(final, want_final, SUMS)
+    got = _gradients(value, forget, gate, state, reset, dy, dstate, run)
+    want = _gradients(value.double(), forget.double(), gate.double(), state.double(), reset, dy, dstate, gated_scan64)
+    for i, (a, e) in enumerate(zip(got, want)):
+        assert_rounded(a, e, 2 * SUMS, f"gradient {i}")
+
+
 def test_gradient_against_differences():
     """The directional derivative of a float32 loss along a random direction, against a central difference
     of the 64-bit definition (error of the difference: about step^2 = 1e-8)."""
