@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2)
     pipe.load(maps, from, i - skipped + kStages - 1, t - (kStages - 1) * cluster, b, c0, a);
     const int n = t0 >= a.length ? 0 : a.length - t0 < kRun ? (int)(a.length - t0) : kRun;
     const bool whole = n == kRun && resets == 0;
-    float2 keep[kRun], lose[kRun], dh[kRun], slope[kRun];  // slope: sigmoid(gate)
+    float2 keep[kRun], lose[kRun], dh[kRun], slope[kRun];  // dy silu(gate), dy silu'(gate)
     const float4 map = whole ? open_run<T, true, true>(tile, tile + kElems, warp * kRun, lane, n, resets, keep, lose)
                              : open_run<T, false, true>(tile, tile + kElems, warp * kRun, lane, n, resets, keep, lose);
     float4 rmap = make_float4(map.x, map.y, 0.0f, 0.0f);
@@ -494,9 +494,11 @@ __global__ void __launch_bounds__(kBwdThreads, 2)
       dh[j] = read_two(tile + 2 * kElems, warp * kRun + j, lane);
       if constexpr (kGate) {
         const float2 q = read_two(tile + 3 * kElems, warp * kRun + j, lane);
-        slope[j] = make_float2(sigmoid_approx(q.x), sigmoid_approx(q.y));
-        dh[j].x *= q.x * slope[j].x;
-        dh[j].y *= q.y * slope[j].y;
+        const float2 sig = make_float2(sigmoid_approx(q.x), sigmoid_approx(q.y));
+        const float2 qs = make_float2(q.x * sig.x, q.y * sig.y);  // silu' = s + gate s (1 - s)
+        slope[j] = make_float2(dh[j].x * fmaf(qs.x, 1.0f - sig.x, sig.x), dh[j].y * fmaf(qs.y, 1.0f - sig.y, sig.y));
+        dh[j].x *= qs.x;
+        dh[j].y *= qs.y;
       }
       rmap.z = keep[j].x * (dh[j].x + rmap.z);
       rmap.w = keep[j].y * (dh[j].y + rmap.w);
@@ -519,42 +521,37 @@ __global__ void __launch_bounds__(kBwdThreads, 2)
     for (int w = 0; w < warp; ++w) h = fold(runs[w * 32 + lane], h);
     for (int w = kWarps - 1; w > warp; --w) mine = fold(back[w * 32 + lane], mine);
     if (cluster == 1 && warp == 0) next[lane] = fold(rmap, mine);
-    float2 prev[kRun];  // h_{t-1} as token t sees it
+    const float2 h_in = h;
+    float2 after[kRun];  // h_t
 #pragma unroll
     for (int j = 0; j < kRun; ++j) {
       if (!whole && j >= n) break;
       if (!whole && (resets >> j & 1u)) h = make_float2(0.0f, 0.0f);
-      prev[j] = h;
       const float2 v = read_two(tile + kElems, warp * kRun + j, lane);
       h.x = fmaf(keep[j].x, h.x, lose[j].x * v.x);
       h.y = fmaf(keep[j].y, h.y, lose[j].y * v.y);
+      after[j] = h;
     }
-    auto finish = [&](int j) {
-      const int token = warp * kRun + j;
-      const float2 v = read_two(tile + kElems, token, lane);
-      if constexpr (kGate) {  // dy h (s + gate s (1 - s))
-        const float2 q = read_two(tile + 3 * kElems, token, lane), dy = read_two(tile + 2 * kElems, token, lane);
-        const float2 s = slope[j];
-        const float2 ht = make_float2(fmaf(keep[j].x, prev[j].x, lose[j].x * v.x), fmaf(keep[j].y, prev[j].y, lose[j].y * v.y));
-        const float2 qs = make_float2(q.x * s.x, q.y * s.y);
-        dgate.write(j, make_float2(dy.x * ht.x * fmaf(qs.x, 1.0f - s.x, s.x), dy.y * ht.y * fmaf(qs.y, 1.0f - s.y, s.y)));
-      }
+    auto finish = [&](int j, float2 prev) {  // prev: h_{t-1} as token t sees it
+      const float2 v = read_two(tile + kElems, warp * kRun + j, lane);
+      if constexpr (kGate) dgate.write(j, make_float2(slope[j].x * after[j].x, slope[j].y * after[j].y));
       const float2 G = make_float2(dh[j].x + mine.x, dh[j].y + mine.y);
       const float2 dv = make_float2(G.x * lose[j].x, G.y * lose[j].y);
       mine.x = keep[j].x * G.x;
       mine.y = keep[j].y * G.y;
       dvalue.write(j, dv);
-      dforget.write(j, make_float2(mine.x * lose[j].x * (prev[j].x - v.x), mine.y * lose[j].y * (prev[j].y - v.y)));
+      dforget.write(j, make_float2(mine.x * lose[j].x * (prev.x - v.x), mine.y * lose[j].y * (prev.y - v.y)));
     };
     if (whole) {
 #pragma unroll
-      for (int j = kRun - 1; j >= 0; --j) finish(j);
+      for (int j = kRun - 1; j >= 0; --j) finish(j, j ? after[j - 1] : h_in);
     } else {
 #pragma unroll
       for (int j = kRun - 1; j >= 0; --j) {
         if (j >= n) continue;
-        finish(j);
-        if (resets >> j & 1u) mine = make_float2(0.0f, 0.0f);
+        const bool fresh = resets >> j & 1u;
+        finish(j, fresh ? make_float2(0.0f, 0.0f) : j ? after[j - 1] : h_in);
+        if (fresh) mine = make_float2(0.0f, 0.0f);
       }
     }
     dvalue.go(-cluster * kTile);
