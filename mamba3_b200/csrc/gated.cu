@@ -95,7 +95,7 @@ template <> struct Two<__nv_bfloat16> {
 template <typename T, int kThreads>
 __device__ __forceinline__ void load_tile(T* tile, const m3_tensor& from, int b, int64_t t0, int c0, int64_t length, int channels) {
   const T* base = static_cast<const T*>(from.data) + b * from.stride[0];
-#pragma unroll 8
+#pragma unroll 16
   for (int i = threadIdx.x; i < kTile * kChannels; i += kThreads) {
     const int t = i / kChannels, c = i % kChannels;
     tile[i] = t0 + t < length && c0 + c < channels ? base[(t0 + t) * from.stride[1] + (c0 + c) * from.stride[2]]
@@ -678,13 +678,17 @@ cudaError_t launch_tiles(K kernel, const m3_gated_args& a, const Maps& maps, int
   // 4 in all the room there is (4 x 2048 x 2048: 47 us in fours, 54 in twos), larger ones, whose exchange takes as long
   // as a tile, up to two CTAs an SM (1 x 65536 x 1536: 308 us in eights, 328 in sixteens; 1 x 32768 x 128: 83 us in
   // sixteens, 136 in eights), and tens where sixteens have no such room (1 x 65536 x 1536: 267 us, backward 647 against
-  // 762). Past 8 CTAs, a cluster's size without conditions, only where two fit an SM.
-  const int per_sm = 227 * 1024 / (smem_bytes(tile, tensors, run_maps, 2) + 1024);
+  // 762). Where the CTAs of eights have all their tiles under way from the start, they take all the room too
+  // (3 x 777 x 1001: 17 us, 26 in fours). Past 8 CTAs, a cluster's size without conditions, only where two fit an SM.
+  // (CTAs that an SM has room for: by shared memory, and by registers at the 128 that both kernels take)
+  const int per_sm = std::min(227 * 1024 / (smem_bytes(tile, tensors, run_maps, 2) + 1024), 65536 / (128 * threads));
   const int most = per_sm > 1 ? kMaxCluster : 8;
   int cluster = 1;
-  while (cluster < most && 2 * cluster <= ntiles &&
-         2 * cluster * blocks <= (int64_t)sm_count() * (cluster < 4 ? per_sm : std::min(per_sm, 2)))
+  while (cluster < most && 2 * cluster <= ntiles) {
+    const bool all_room = cluster < 4 || (cluster == 4 && 8 * kStages >= ntiles);
+    if (2 * cluster * blocks > (int64_t)sm_count() * (all_room ? per_sm : std::min(per_sm, 2))) break;
     cluster *= 2;
+  }
   if (cluster == 8 && most > 8 && 10 <= ntiles && 10 * blocks <= 2 * (int64_t)sm_count()) cluster = 10;
   const int smem = smem_bytes(tile, tensors, run_maps, cluster);
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
