@@ -154,8 +154,8 @@ def gated_step(value: torch.Tensor, forget: torch.Tensor, state: torch.Tensor, g
     if torch.is_grad_enabled() and (value.requires_grad or forget.requires_grad or state.requires_grad
                                     or (gate is not None and gate.requires_grad)):
         raise ValueError("gated_step does not support gradients on CUDA; use gated_scan")
-    y = torch.empty(shape, device=device, dtype=dtype)
-    new = torch.empty(shape, device=device, dtype=torch.float32) if out_state is None else out_state
+    y = torch.empty(shape[0], shape[1], device=device, dtype=dtype)  # plain ints: half the time of a torch.Size
+    new = torch.empty_like(state) if out_state is None else out_state
     _ext.gated_step(value, forget, gate, state, y=y, out_state=new)
     return y, new
 
