@@ -375,11 +375,41 @@ __device__ __forceinline__ void arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+// Whether the barrier's phase is over, without waiting.
+__device__ __forceinline__ bool passed(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
 __device__ __forceinline__ void mma_if(uint32_t leader, uint32_t to, uint64_t da, uint64_t db, uint32_t id, uint32_t adds) {
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
       "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(to),
       "l"(da), "l"(db), "r"(id), "r"(adds), "r"(leader));
+}
+__device__ __forceinline__ uint32_t elect() {
+  uint32_t leader;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+  return leader;
+}
+__device__ __forceinline__ void expect_if(uint32_t leader, uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}\n" ::"r"(bar),
+      "r"(bytes), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void copy_if(uint32_t leader, uint32_t to, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n\t}\n" ::"r"(
+          to),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar), "r"(leader)
+      : "memory");
 }
 __device__ __forceinline__ void commit_if(uint32_t leader, uint32_t bar) {
   asm volatile(
@@ -413,12 +443,11 @@ __global__ void __launch_bounds__(Many<kN>::kThreads, 1)
   uint8_t* smem = raw + (base - umma::smem_u32(raw));
   const uint32_t bars = base + M::kOffBars;
   auto full = [&](int s) { return bars + 8u * (s & (kStages - 1)); };
-  auto sums_full = [&](int g) { return bars + 8u * (2 * kStages + (g & (kSumsRing - 1))); };
-  auto sums_empty = [&](int g) { return bars + 8u * (2 * kStages + kSumsRing + (g & (kSumsRing - 1))); };
-  auto came = [&](int s) { return bars + 8u * (2 * kStages + 2 * kSumsRing + (s & (kRing - 1))); };
-  auto read = [&](int s) { return bars + 8u * (2 * kStages + 2 * kSumsRing + kRing + (s & (kRing - 1))); };
-  auto freed = [&](int s) { return bars + 8u * (2 * kStages + 2 * kSumsRing + 2 * kRing + (s & (kRing - 1))); };
-  const uint32_t drained = bars + 8u * (2 * kStages + 2 * kSumsRing + 3 * kRing), slot = drained + 8u;
+  auto sums_full = [&](int g) { return bars + 8u * (kStages + (g & (kSumsRing - 1))); };
+  auto sums_empty = [&](int g) { return bars + 8u * (kStages + kSumsRing + (g & (kSumsRing - 1))); };
+  auto came = [&](int s) { return bars + 8u * (kStages + 2 * kSumsRing + (s & (kRing - 1))); };
+  auto freed = [&](int s) { return bars + 8u * (kStages + 2 * kSumsRing + kRing + (s & (kRing - 1))); };
+  const uint32_t drained = bars + 8u * (kStages + 2 * kSumsRing + 2 * kRing), slot = drained + 8u;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   int rank = 0;
   if (split > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -436,7 +465,6 @@ __global__ void __launch_bounds__(Many<kN>::kThreads, 1)
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(full(i)), "r"(4));
     for (int i = 0; i < kRing; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(came(i)));
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(read(i)), "r"(4));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(freed(i)));
     }
     for (int i = 0; i < kSumsRing; ++i) {
@@ -573,44 +601,31 @@ __global__ void __launch_bounds__(Many<kN>::kThreads, 1)
       }
       umma::fence_async_smem();
       __syncwarp();
-      if (lane == 0) {  // one arrival a warp: a barrier takes them one by one
-        arrive(full(s));
-        arrive(read(s));
-      }
+      if (lane == 0) arrive(full(s));  // one arrival a warp: a barrier takes them one by one
     }
   } else if (warp == kProducers / 32 + 1) {
-    if (lane == 0) {  // the copies; a stage's barrier completes without bytes where TMA cannot read either
-      bool ok = true;
-      int s = 0;
-      for (; s < stages && ok; ++s) {
-        if (s >= kRing) {
-          ok = umma::mbar_wait(read(s), (uint32_t)(s / kRing - 1) & 1u);
-          if (ok) ok = umma::mbar_wait(freed(s), (uint32_t)(s / kRing - 1) & 1u);  // the MMAs are done with its x
-          if (!ok) break;
-        }
-        umma::mbar_expect_tx(came(s), (code_tiles ? M::kCodes : 0) + (x_tiles ? M::kX : 0));
-        const int c = first + s * kStage;
-        if (code_tiles)
-          asm volatile(
-              "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-                  base + M::kOffCodes + (s & (kRing - 1)) * M::kCodes),
-              "l"(reinterpret_cast<uint64_t>(&code_map)), "r"(c / 2), "r"((int)o0), "r"(came(s))
-              : "memory");
-        if (x_tiles)
-          asm volatile(
-              "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-                  base + M::kOffX + (s & (kRing - 1)) * M::kX),
-              "l"(reinterpret_cast<uint64_t>(&x_map)), "r"(c), "r"((int)rows0), "r"(came(s))
-              : "memory");
+    // The copies; a stage's barrier completes without bytes where TMA cannot read either. A stage that the MMAs are done
+    // with has been read by the teams too. (In step, as the warp of the MMAs: one lane took 0.3 us a stage.)
+    const uint32_t leader = elect();
+    const uint32_t bytes = (code_tiles ? M::kCodes : 0) + (x_tiles ? M::kX : 0);
+    bool ok = true;
+    int s = 0;
+    for (; s < stages; ++s) {
+      if (s >= kRing) {
+        ok = __all_sync(0xffffffffu, umma::mbar_wait(freed(s), (uint32_t)(s / kRing - 1) & 1u));
+        if (!ok) break;
       }
-      if (!ok)  // gave up: the copies under way land before the block's shared memory goes
-        for (int i = max(0, s - kRing); i < s; ++i) umma::mbar_wait(came(i), (uint32_t)(i / kRing) & 1u);
+      expect_if(leader, came(s), bytes);
+      const int c = first + s * kStage;
+      if (code_tiles) copy_if(leader, base + M::kOffCodes + (s & (kRing - 1)) * M::kCodes, &code_map, c / 2, (int)o0, came(s));
+      if (x_tiles) copy_if(leader, base + M::kOffX + (s & (kRing - 1)) * M::kX, &x_map, c, (int)rows0, came(s));
     }
+    if (!ok)  // gave up: the copies under way land before the block's shared memory goes
+      for (int i = max(0, s - kRing); i < s; ++i) umma::mbar_wait(came(i), (uint32_t)(i / kRing) & 1u);
   } else if (warp == kProducers / 32) {
     // The chain that all else waits for: no division, one commit a stage and one a group. The whole warp goes through
     // it and one lane's instructions count, so that addresses and descriptors are the warp's, in uniform registers.
-    uint32_t leader;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+    const uint32_t leader = elect();
     const uint32_t id = umma::idesc(kManyOuts, kN, std::is_same<T, __nv_bfloat16>::value, false, false);
     const uint32_t acc0 = __shfl_sync(0xffffffffu, tmem, 0);
     const uint64_t da0 = umma::sdesc(base, 16, 1024), db0 = umma::sdesc(base + M::kOffX, 16, 1024);
@@ -621,16 +636,21 @@ __global__ void __launch_bounds__(Many<kN>::kThreads, 1)
     };
     // A stage is half a group, a group or two; columns past the row are zeros of x.
     const int parts = a.group == 32 ? 2 : 1, stages_of = a.group == 128 ? 2 : 1;
-    bool ok = true;
+    auto empty = [&](int g) { return g < kSumsRing || g >= groups || passed(sums_empty(g), (uint32_t)(g / kSumsRing - 1) & 1u); };
+    auto begin = [&](int g) { return g < kSumsRing || umma::mbar_wait(sums_empty(g), (uint32_t)(g / kSumsRing - 1) & 1u); };
+    bool ok = true, come = false, room = true;  // the stage's operands, its group's accumulator: looked at a stage ahead
     int g = 0;
     for (int s = 0; s < stages && ok; ++s) {
-      ok = umma::mbar_wait(full(s), (uint32_t)(s / kStages) & 1u);
-      auto begin = [&]() { return g < kSumsRing || umma::mbar_wait(sums_empty(g), (uint32_t)(g / kSumsRing - 1) & 1u); };
       const bool opens = stages_of == 1 || (s & 1) == 0, closes = stages_of == 1 || (s & 1) == 1 || s + 1 == stages;
-      if (opens) ok = ok && begin();
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
+      if (!__all_sync(0xffffffffu, come && room)) {
+        ok = umma::mbar_wait(full(s), (uint32_t)(s / kStages) & 1u);
+        if (opens) ok = ok && begin(g);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+      }
       umma::fence_after();
+      come = s + 1 < stages && passed(full(s + 1), (uint32_t)((s + 1) / kStages) & 1u);
+      room = closes ? empty(g + parts) : true;
       const uint64_t da = umma::sdesc_at(da0, (s & (kStages - 1)) * M::kA), db = umma::sdesc_at(db0, (s & (kRing - 1)) * M::kX);
       uint32_t to = acc0 + (g & (kSumsRing - 1)) * kN;
       product(to, da, db, !opens);
@@ -641,7 +661,7 @@ __global__ void __launch_bounds__(Many<kN>::kThreads, 1)
           commit_if(leader, freed(s));
           break;
         }
-        ok = __all_sync(0xffffffffu, begin());
+        ok = __all_sync(0xffffffffu, begin(g));
         if (!ok) break;
         umma::fence_after();
         to = acc0 + (g & (kSumsRing - 1)) * kN;
