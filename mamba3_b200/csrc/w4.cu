@@ -252,7 +252,10 @@ __host__ __device__ __forceinline__ bool x_in_units(const m3_w4_args& a) {
 
 // ---- up to 8 rows --------------------------------------------------------------------------------
 // A stream of codes: one CTA for 16 outputs, its warps share the columns out, slab by slab, and meet in shared memory.
-// x, a few KB, comes from L1 as the products want it.
+// x, a few KB, comes from L1 as the products want it. 10768 x 2560, groups of 128: 6.3 us at one row (2.2 TB/s of codes),
+// 7.1 at eight, groups of 64 and 32: 7.7 and 9.5; 8192 x 8192: 17.8; what bounds it at these sizes is a wave's latency,
+// the launch, the first codes and the meeting of the warps. Scales widened where they are fetched cost 1.6 us of 8.
+// Rows of codes that are no whole words (10768 x 2561): 21.
 constexpr int kMostWarps = 16;
 
 template <typename T, int kWords, bool kFast, bool kZeros>
@@ -270,8 +273,12 @@ __global__ void __launch_bounds__(32 * kMostWarps) w4_few_kernel(const m3_w4_arg
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const bool units = x_in_units(a);
   // (a thread's type of scales: 16 bits in the fast form)
-  auto value = [&](uint32_t v) { return kFast ? (weight.type == M3_BF16 ? __uint_as_float(v << 16) : __half2float(__ushort_as_half((uint16_t)v))) : widen(v, weight.type); };
-  const T* row = static_cast<const T*>(a.x.data) + min(g, (int)a.rows - 1) * a.x.stride[0];  // past the last row: the last, not written
+  auto value = [&](uint32_t v) {
+    if constexpr (!kFast) return widen(v, weight.type);
+    return weight.type == M3_BF16 ? __uint_as_float(v << 16) : __half2float(__ushort_as_half((uint16_t)v));
+  };
+  // (past the last row: the last one again, not written)
+  const T* row = static_cast<const T*>(a.x.data) + min(g, (int)a.rows - 1) * a.x.stride[0];
   typename W::Slab held[kAhead];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) weight.fetch(warp + i * warps, held[i]);
@@ -352,10 +359,11 @@ __global__ void __launch_bounds__(32 * kMostWarps) w4_few_kernel(const m3_w4_arg
 // four warps read it, a thread an output, and add it, scaled, to sums in registers, in float32. Where the outputs are
 // too few for the SMs, a cluster of CTAs shares the columns out and its partial sums meet through distributed shared
 // memory.
-// What bounds it is the chain of waits, issue and commits of the MMA warp, about 0.3 us a stage, with 85 CTAs for 148
-// SMs: 10768 x 2560, groups of 128, takes 15.4, 16.3 and 17.9 us at 16, 32 and 64 rows (23 with zero points, 34 in
-// groups of 32), 50 at 256; 2560 x 5120 takes 12 at 64. One lane in a branch of its own, whose descriptors go through
-// vector registers, took 24 at 64 rows; stages of 128 columns 19.5; the warp-level instruction 15.3, 19.8 and 31.
+// What bounds it is the chain of waits, issue and commits of the MMA warp, about 0.25 us a stage, with 85 CTAs for 148
+// SMs: 10768 x 2560, groups of 128, takes 14.2, 15.8 and 16.7 us at 16, 32 and 64 rows (20 with zero points, 26 in
+// groups of 32), 47 at 256; 2560 x 5120 takes 12 at 64. Before the issuing warps went in step (one lane in a branch of
+// its own sends addresses and descriptors through vector registers) 64 rows took 24; stages of 128 columns took 19.5
+// against 17.9 then; the warp-level instruction took 15.3, 19.8 and 31 at 16, 32 and 64 rows.
 constexpr int kManyOuts = 128, kStage = 64;  // outputs of a CTA, columns of a stage
 constexpr int kStages = 4, kRing = 8;        // of codes as 16-bit values; of codes and x as they come (powers of two)
 constexpr int kTeams = 3, kProducers = 128 * kTeams;
@@ -698,33 +706,34 @@ __global__ void __launch_bounds__(Many<kN>::kThreads, 1)
       z_held[i] = kZeros ? fetch(zero_at, a.zeros.stride[1], i) : 0u;
     }
     bool ok = true;
-    for (int g0 = 0; g0 < groups && ok; g0 += kAhead)
+    for (int g0 = 0; g0 < groups && ok; g0 += kAhead) {
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int g = g0 + i;
-      if (g >= groups) break;
-      const float s = value(s_held[i]), z = value(z_held[i]) - 8.0f;
-      s_held[i] = fetch(scale_at, a.scales.stride[1], g + kAhead);
-      if (kZeros) z_held[i] = fetch(zero_at, a.zeros.stride[1], g + kAhead);
-      ok = __all_sync(0xffffffffu, umma::mbar_wait(sums_full(g), (uint32_t)(g / kSumsRing) & 1u));
-      if (!ok) break;
-      umma::fence_after();
-      const uint32_t from = tmem + (g & (kSumsRing - 1)) * kN + col0 + ((uint32_t)(quarter * 32) << 16);
+      for (int i = 0; i < kAhead; ++i) {
+        const int g = g0 + i;
+        if (g >= groups) break;
+        const float s = value(s_held[i]), z = value(z_held[i]) - 8.0f;
+        s_held[i] = fetch(scale_at, a.scales.stride[1], g + kAhead);
+        if (kZeros) z_held[i] = fetch(zero_at, a.zeros.stride[1], g + kAhead);
+        ok = __all_sync(0xffffffffu, umma::mbar_wait(sums_full(g), (uint32_t)(g / kSumsRing) & 1u));
+        if (!ok) break;
+        umma::fence_after();
+        const uint32_t from = tmem + (g & (kSumsRing - 1)) * kN + col0 + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll
-      for (int n0 = 0; n0 < M::kCols; n0 += kPart) {
-        uint32_t r[kPart], u[kPart];
-        load(from + n0, r);
-        if (kZeros) load(from + kSumsRing * kN + n0, u);
-        umma::tmem_wait_ld();
+        for (int n0 = 0; n0 < M::kCols; n0 += kPart) {
+          uint32_t r[kPart], u[kPart];
+          load(from + n0, r);
+          if (kZeros) load(from + kSumsRing * kN + n0, u);
+          umma::tmem_wait_ld();
 #pragma unroll
-        for (int e = 0; e < kPart; ++e) {
-          const float d = __uint_as_float(r[e]);
-          acc[n0 + e] = fmaf(s, kZeros ? fmaf(-z, __uint_as_float(u[e]), d) : d, acc[n0 + e]);
+          for (int e = 0; e < kPart; ++e) {
+            const float d = __uint_as_float(r[e]);
+            acc[n0 + e] = fmaf(s, kZeros ? fmaf(-z, __uint_as_float(u[e]), d) : d, acc[n0 + e]);
+          }
         }
+        umma::fence_before();
+        __syncwarp();
+        if (lane == 0) arrive(sums_empty(g));
       }
-      umma::fence_before();
-      __syncwarp();
-      if (lane == 0) arrive(sums_empty(g));
     }
   }
   __syncwarp();

@@ -111,6 +111,14 @@ def test_unaligned_rows_between_other_values(rows, offset):
     _check(x, packed, scales, zero, 32, linear_w4(x, packed, scales, zero, group_size=32))
 
 
+@pytest.mark.parametrize("rows", [5, 20, 40])
+def test_rows_that_overlap(rows):
+    """Windows over one signal: rows 8 columns apart."""
+    codes, scales, zero = _weight(96, 256, 64, False, torch.bfloat16)
+    x = torch.randn(8 * rows + 256, device="cuda").to(torch.bfloat16).as_strided((rows, 256), (8, 1))
+    _check(x, codes, scales, zero, 64, linear_w4(x, codes, scales, zero, group_size=64))
+
+
 def test_zero_scales_and_nonfinite_rows():
     codes, scales, zero = _weight(64, 256, 64, False, torch.bfloat16)
     scales[5] = 0.0
