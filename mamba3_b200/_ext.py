@@ -575,7 +575,7 @@ def gated_scan_backward(value, forget, gate, reset, carry, dy, dstate, want_init
     """``m3_gated_scan_bwd``: ``(dvalue, dforget, dgate or None, dinitial or None)``."""
     lib = load()
     batch, length, channels = value.shape
-    dvalue = torch.empty(value.shape, device=value.device, dtype=value.dtype)
+    dvalue = torch.empty(batch, length, channels, device=value.device, dtype=value.dtype)
     dforget = torch.empty_like(dvalue)
     dgate = None if gate is None else torch.empty_like(dvalue)
     dinitial = torch.empty(batch, channels, device=value.device, dtype=torch.float32) if want_initial else None

@@ -74,8 +74,9 @@ class _GatedScan(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, value, forget, gate, state, reset):
-        y = torch.empty(value.shape, device=value.device, dtype=value.dtype)
-        out = torch.empty(value.shape[0], value.shape[2], device=value.device, dtype=torch.float32)
+        batch, length, channels = value.shape
+        y = torch.empty(batch, length, channels, device=value.device, dtype=value.dtype)
+        out = torch.empty(batch, channels, device=value.device, dtype=torch.float32)
         carry = _ext.gated_carry(value)
         _ext.gated_scan_forward(value, forget, gate, reset, state, y=y, out_state=out, carry=carry)
         ctx.save_for_backward(value, forget, gate, reset, carry)
@@ -115,7 +116,7 @@ def gated_scan(value: torch.Tensor, forget: torch.Tensor, gate: torch.Tensor | N
                                     or (gate is not None and gate.requires_grad)
                                     or (initial_state is not None and initial_state.requires_grad)):
         return _GatedScan.apply(value, forget, gate, initial_state, reset)
-    y = torch.empty(value.shape, device=value.device, dtype=value.dtype)
+    y = torch.empty(batch, length, channels, device=value.device, dtype=value.dtype)
     state = torch.empty(batch, channels, device=value.device, dtype=torch.float32)
     _ext.gated_scan_forward(value, forget, gate, reset, initial_state, y=y, out_state=state)
     return y, state
