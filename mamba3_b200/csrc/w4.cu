@@ -879,8 +879,9 @@ extern "C" int m3_linear_w4(const m3_w4_args* args, void* stream) {
   const m3_w4_args& a = *args;
   if (a.rows <= 0 || a.out_dim <= 0 || a.in_dim <= 0)
     return report_error(M3_ERR_SHAPE, "m3_linear_w4: rows, out_dim and in_dim must be positive");
-  if (a.rows > 64 * 65535 || a.out_dim > INT32_MAX || a.in_dim > INT32_MAX)
-    return report_error(M3_ERR_SHAPE, "m3_linear_w4: rows above 64 * 65535, or out_dim or in_dim above 2^31 - 1");
+  constexpr int64_t kMost = INT32_MAX - 4096;  // columns a few stages past the row's end still count in 32 bits
+  if (a.rows > 64 * 65535 || a.out_dim > kMost || a.in_dim > kMost)
+    return report_error(M3_ERR_SHAPE, "m3_linear_w4: rows above 64 * 65535, or out_dim or in_dim above 2^31 - 4097");
   if (a.group != 32 && a.group != 64 && a.group != 128)
     return report_error(M3_ERR_SHAPE, "m3_linear_w4: group must be 32, 64 or 128");
   if (!a.x.data || !a.codes.data || !a.scales.data || !a.y.data)
