@@ -13,6 +13,7 @@
 //   dstate_0  = In_0.
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "common.cuh"
 #include "umma.cuh"
@@ -43,6 +44,8 @@ constexpr int kTile = 64;        // tokens a tile: the training forward keeps th
 constexpr int kChannels = 64;    // channels a CTA; a thread has two neighbouring ones
 constexpr float kFloor = 1e-37f; // least product of decays without a reset: see fold()
 
+template <typename T> constexpr bool kFine = std::is_same<T, float>::value;
+
 // exp2 and reciprocal of the special-function unit, results below 2^-126 taken as 0. The compiler's __expf and
 // __fdividef add the handling of such values, which no use here can tell apart.
 __device__ __forceinline__ float rcp_approx(float x) {
@@ -51,17 +54,44 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return y;
 }
 
-// f = sigmoid(x) and 1 - f = sigmoid(-x), both to a few units in the last place; x below -80 is taken as -80
-// (f = 2e-35), so that exp stays finite; NaN stays NaN.
-__device__ __forceinline__ void keep_lose(float x, float& keep, float& lose) {
-  float c;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(x), "f"(-80.0f));
-  const float e = ex2_approx(c * -kLog2e);
-  keep = rcp_approx(1.0f + e);
+// With float32 inputs (kExact) a sigmoid is good to about one unit in the last place: the rounding of c log2(e), which
+// for c = 8 is worth five units of its exponential, is recovered by fma, and the reciprocal gets a Newton step.
+// Decays near 1 hold an error for as many tokens as they hold a value, so it shows in the state. 16-bit inputs, whose
+// outputs are rounded to 8 or 11 bits, take the two instructions as they are.
+template <bool kExact> __device__ __forceinline__ float exp_minus(float c) {
+  const float t = c * -kLog2e, e = ex2_approx(t);
+  if constexpr (!kExact) return e;
+  constexpr float kLow = (float)(1.4426950408889634 - (double)kLog2e), kLn2 = 0.6931471805599453f;
+  return fmaf(e, kLn2 * fmaf(c, -kLow, fmaf(c, -kLog2e, -t)), e);
+}
+template <bool kExact> __device__ __forceinline__ float reciprocal(float d) {
+  const float r = rcp_approx(d);
+  return kExact ? fmaf(r, fmaf(-d, r, 1.0f), r) : r;
+}
+__device__ __forceinline__ float at_least(float x, float least) {  // NaN stays NaN
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(x), "f"(least));
+  return x;
+}
+__device__ __forceinline__ float at_most(float x, float most) {
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(x), "f"(most));
+  return x;
+}
+
+// f = sigmoid(x) and 1 - f = sigmoid(-x); x below -80 is taken as -80 (f = 2e-35), so that exp stays finite; NaN stays
+// NaN. (kExact: past 100, where exp(-x) is 0, the differences of infinities are kept out.)
+template <bool kExact> __device__ __forceinline__ void keep_lose(float x, float& keep, float& lose) {
+  float c = at_least(x, -80.0f);
+  if (kExact) c = at_most(c, 100.0f);
+  const float e = exp_minus<kExact>(c);
+  keep = reciprocal<kExact>(1.0f + e);
   lose = e * keep;
 }
 
-__device__ __forceinline__ float sigmoid_approx(float x) { return rcp_approx(1.0f + ex2_approx(x * -kLog2e)); }
+// sigmoid(x), 0 below -88.
+template <bool kExact> __device__ __forceinline__ float sigmoid(float x) {
+  if (kExact) x = at_most(at_least(x, -88.0f), 100.0f);
+  return reciprocal<kExact>(1.0f + exp_minus<kExact>(x));
+}
 
 // A run of tokens as a map of the state before it: h -> a h + h0. a is exactly 0 where a reset lies in the run,
 // and then nothing of h passes, not even an infinity or NaN; otherwise a product of decays is kept at kFloor or
@@ -315,8 +345,8 @@ __device__ __forceinline__ float4 open_run(const T* forget, const T* value, int 
     }
     const float2 f = read_two(forget, token + j, lane), v = read_two(value, token + j, lane);
     float2 lose;
-    keep_lose(f.x, keep[j].x, lose.x);
-    keep_lose(f.y, keep[j].y, lose.y);
+    keep_lose<kFine<T>>(f.x, keep[j].x, lose.x);
+    keep_lose<kFine<T>>(f.y, keep[j].y, lose.y);
     const float2 in = make_float2(lose.x * v.x, lose.y * v.y);
     other[j] = kLose ? lose : in;
     if (!kWhole && (resets >> j & 1u)) {
@@ -405,8 +435,8 @@ __global__ void __launch_bounds__(kFwdThreads, 4)
       float2 out = h;
       if constexpr (kGate) {
         const float2 q = read_two(tile + 2 * kElems, warp * kRun + j, lane);
-        out.x *= q.x * sigmoid_approx(q.x);
-        out.y *= q.y * sigmoid_approx(q.y);
+        out.x *= q.x * sigmoid<kFine<T>>(q.x);
+        out.y *= q.y * sigmoid<kFine<T>>(q.y);
       }
       y.write(j, out);
     };
@@ -502,7 +532,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2)
       dh[j] = read_two(tile + 2 * kElems, warp * kRun + j, lane);
       if constexpr (kGate) {
         const float2 q = read_two(tile + 3 * kElems, warp * kRun + j, lane);
-        const float2 sig = make_float2(sigmoid_approx(q.x), sigmoid_approx(q.y));
+        const float2 sig = make_float2(sigmoid<kFine<T>>(q.x), sigmoid<kFine<T>>(q.y));
         const float2 qs = make_float2(q.x * sig.x, q.y * sig.y);  // silu' = s + gate s (1 - s)
         slope[j] = make_float2(dh[j].x * fmaf(qs.x, 1.0f - sig.x, sig.x), dh[j].y * fmaf(qs.y, 1.0f - sig.y, sig.y));
         dh[j].x *= qs.x;
@@ -609,9 +639,9 @@ __global__ void __launch_bounds__(128) gated_step_kernel(const m3_gated_args a) 
 #pragma unroll
   for (int e = 0; e < kWide; ++e) {
     float keep, lose;
-    keep_lose(f[e], keep, lose);
+    keep_lose<kFine<T>>(f[e], keep, lose);
     h[e] = fmaf(keep, reset ? 0.0f : h[e], lose * v[e]);
-    y[e] = a.gate.data ? h[e] * (q[e] * sigmoid_approx(q[e])) : h[e];
+    y[e] = a.gate.data ? h[e] * (q[e] * sigmoid<kFine<T>>(q[e])) : h[e];
   }
   float* op = static_cast<float*>(a.out_state.data) + b * a.out_state.stride[0] + c * a.out_state.stride[1];
   T* yp = at(a.y);
