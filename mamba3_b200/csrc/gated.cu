@@ -730,7 +730,10 @@ cudaError_t launch_tiles(K kernel, const m3_gated_args& a, const Maps& maps, int
   }
   if (cluster == 8 && most > 8 && 10 <= ntiles && 10 * blocks <= 2 * (int64_t)sm_count()) cluster = 10;
   const int smem = smem_bytes(tile, tensors, run_maps, cluster);
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  // The limit is the kernel's, not the launch's: the largest cluster's always, or another thread with a shorter sequence
+  // could lower it between this call and the launch below.
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       smem_bytes(tile, tensors, run_maps, kMaxCluster));
   if (e != cudaSuccess) return e;
   if (cluster > 8) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);

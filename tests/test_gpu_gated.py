@@ -9,6 +9,8 @@ rounding to the tensor's type."""
 
 from __future__ import annotations
 
+import threading
+
 import pytest
 import torch
 
@@ -282,3 +284,29 @@ def test_module_on_the_gpu_matches_the_cpu():
         assert_rounded(last[:, 0], want[:, 99].detach(), 1e-5)
         again, _ = model.step(x[:, 99:].cuda(), cache, in_place=True)
         assert torch.equal(again, last)
+
+
+def test_threads_with_different_shapes():
+    """Calls of one kernel from several host threads, with clusters of 16 and of one CTA: the launches need
+    different amounts of shared memory."""
+    calls = [[t.contiguous() for t in torch.randn(3, 1, length, 64, device="cuda").bfloat16().unbind(0)]
+             for length in (2048, 64)]
+    want = [gated_scan(*x)[0] for x in calls]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(x, expected):
+        try:
+            for _ in range(10000):
+                y, _ = gated_scan(*x)
+            if not torch.equal(y, expected):
+                failed.append("another result")
+        except RuntimeError as error:
+            failed.append(str(error))
+
+    threads = [threading.Thread(target=work, args=(calls[i % 2], want[i % 2])) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
