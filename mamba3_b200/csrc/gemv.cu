@@ -17,6 +17,7 @@ namespace {
 
 constexpr int kGemvThreads = 256;
 constexpr int kRowsPerWarp = 1;
+constexpr int kMostColumns = 16384;
 constexpr int kUnroll = 10;  // 256-element blocks whose loads are issued together (I <= 2560: all)
 
 template <typename T> __device__ __forceinline__ void fma8(float& acc, uint4 w, uint4 x) {
@@ -102,7 +103,8 @@ __global__ void __launch_bounds__(kGemvThreads) gemv_kernel(const m3_gemv_args a
 
 template <typename T, int M> cudaError_t launch_m(const m3_gemv_args& a, cudaStream_t stream) {
   const size_t smem = (size_t)M * a.in_dim * sizeof(T);
-  cudaError_t e = cudaFuncSetAttribute(gemv_kernel<T, M>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  // the widest row's limit: one that followed the call could be lowered by another thread before the launch
+  cudaError_t e = cudaFuncSetAttribute(gemv_kernel<T, M>, cudaFuncAttributeMaxDynamicSharedMemorySize, M * kMostColumns * (int)sizeof(T));
   if (e != cudaSuccess) return e;
   const int64_t per_cta = (kGemvThreads / 32) * kRowsPerWarp;
   cudaLaunchConfig_t cfg = {};
@@ -135,7 +137,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 extern "C" int m3_gemv(const m3_gemv_args* args, void* stream) {
   if (args == nullptr) return m3::report_error(M3_ERR_ARGUMENT, "null argument struct");
   const m3_gemv_args& a = *args;
-  if (a.rows < 1 || a.rows > 4 || a.out_dim <= 0 || a.in_dim <= 0 || a.in_dim % 8 != 0 || a.in_dim > 16384)
+  if (a.rows < 1 || a.rows > 4 || a.out_dim <= 0 || a.in_dim <= 0 || a.in_dim % 8 != 0 || a.in_dim > m3::kMostColumns)
     return m3::report_error(M3_ERR_SHAPE, "m3_gemv: 1 to 4 rows, in_dim a positive multiple of 8 (<= 16384)");
   if (!a.x.data || !a.w.data || !a.y.data || a.x.dtype == M3_F32 || a.w.dtype != a.x.dtype || a.y.dtype != a.x.dtype)
     return m3::report_error(M3_ERR_DTYPE, "m3_gemv: x, w and y must share one 16-bit dtype");

@@ -288,16 +288,17 @@ template <typename T, int R>
 static cudaError_t launch_simt_r(const m3_scan_args& a, cudaStream_t stream) {
   const int N = a.d_state, P = a.head_dim, S = a.num_angles;
   dim3 grid(a.heads, a.batch);
+  constexpr size_t kMaxSmem = 227 * 1024;  // also every launch's limit: one that followed the call could be lowered by
+                                           // another thread before the launch
   auto try_rows = [&](auto rows_tag) -> cudaError_t {
     constexpr int ROWS = decltype(rows_tag)::value;
     const SimtLayout lay = simt_layout(ROWS, ROWS / R, N, P, S);
     auto kern = scan_simt_kernel<T, R, ROWS>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lay.total);
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem);
     if (e != cudaSuccess) return e;
     kern<<<grid, 256, lay.total, stream>>>(a);
     return cudaGetLastError();
   };
-  constexpr size_t kMaxSmem = 227 * 1024;
   if (simt_layout(64, 64 / R, N, P, S).total <= kMaxSmem) return try_rows(std::integral_constant<int, 64>{});
   return try_rows(std::integral_constant<int, 32>{});
 }

@@ -679,8 +679,10 @@ static int64_t ssd_scratch_floats(const m3_ssd_args& a, bool bwd) {
   return small + (bwd ? slots * a.head_dim * a.d_state : 0);
 }
 
-template <typename K> static cudaError_t set_smem(K kern, size_t bytes) {
-  return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+// The limit is the kernel's, not the launch's: all that a block may have, since one that followed the call could be lowered
+// by another thread's call before the launch.
+template <typename K> static cudaError_t raise_smem_limit(K kern) {
+  return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
 }
 
 static int ssd_launch(const m3_ssd_args* args, void* stream_, bool bwd) {
@@ -698,9 +700,9 @@ static int ssd_launch(const m3_ssd_args* args, void* stream_, bool bwd) {
   float* gs = ws + slots;
   float* grads = ws + (2 * slots + 3) / 4 * 4;
   const dim3 chunk_grid((unsigned)nchunk, a.heads, a.batch), bh_grid(a.heads, a.batch);
-  cudaError_t e = set_smem(ssdt::chunk_delta_kernel, ssdt::delta_smem(N, P));
+  cudaError_t e = raise_smem_limit(ssdt::chunk_delta_kernel);
   if (!bwd) {
-    if (e == cudaSuccess) e = set_smem(ssdt::chunk_output_kernel, ssdt::output_smem(N, P));
+    if (e == cudaSuccess) e = raise_smem_limit(ssdt::chunk_output_kernel);
     if (e == cudaSuccess) {
       ssdt::chunk_delta_kernel<<<chunk_grid, ssdt::kThreads, ssdt::delta_smem(N, P), stream>>>(
           a, 0, static_cast<float*>(a.chunk_states.data), lam);
@@ -709,7 +711,7 @@ static int ssd_launch(const m3_ssd_args* args, void* stream_, bool bwd) {
       e = cudaGetLastError();
     }
   } else {
-    if (e == cudaSuccess) e = set_smem(ssdt::chunk_grads_kernel, ssdt::grads_smem(N, P));
+    if (e == cudaSuccess) e = raise_smem_limit(ssdt::chunk_grads_kernel);
     if (e == cudaSuccess) {
       ssdt::chunk_delta_kernel<<<chunk_grid, ssdt::kThreads, ssdt::delta_smem(N, P), stream>>>(a, 1, grads, lam);
       ssdt::grad_scan_kernel<<<bh_grid, ssdt::kThreads, 0, stream>>>(a, grads, lam, gs);

@@ -1110,7 +1110,8 @@ static cudaError_t launch_step_r(const m3_step_args& a, cudaStream_t stream) {
   const size_t smem = (128 + 3 * (size_t)R * N + 2 * R) * sizeof(float);
   auto go = [&](auto kern) -> cudaError_t {
     if (smem > 48 * 1024) {
-      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      // (not `smem`: another thread could lower the limit to its own call's before the launch)
+      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
       if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t cfg = {};
