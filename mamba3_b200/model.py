@@ -643,7 +643,9 @@ class _CudaGraphDecoder:
         if model.training:
             raise ValueError("cuda_graph requires model.eval()")
         self.model = model
+        # what the graph reads by address outside its own pool stays alive with it, whatever becomes of the model
         self.parameters = tuple(model.parameters())
+        self.buffers = tuple(model.buffers())  # 4-bit weights among them
         self.parameter_signature = self._parameter_signature()
         device = parameter.device
         self.input = torch.zeros(batch_size, 1, model.d_model, device=device, dtype=parameter.dtype)

@@ -8,6 +8,9 @@ rounding to the output's type."""
 
 from __future__ import annotations
 
+import gc
+import weakref
+
 import pytest
 import torch
 
@@ -183,3 +186,26 @@ def test_quantised_model_runs_the_dequantised_weights(causal):
                 step, cache = model.step(x[:, t:t + 1], cache)
                 assert float((y.float() - step.float()).norm() / step.float().norm()) < 1e-2
                 assert float((step[:, 0].float() - want[:, t].float()).norm() / want[:, t].float().norm()) < 3e-2
+
+
+def test_a_decoder_keeps_the_weights_that_its_graph_reads():
+    """Projections are replaced, and the old ones dropped, after the capture."""
+    torch.manual_seed(0)
+    model = Mamba3(256, d_state=128, depth=2).cuda().to(torch.bfloat16).eval()
+    quantize_projections(model, group_size=64)
+    x = torch.randn(2, 1, 256, device="cuda", dtype=torch.bfloat16)
+    decoder = model.cuda_graph(batch_size=2)
+    read = [weakref.ref(t) for t in model.buffers()]
+    want = decoder(x).clone()
+    decoder.validate()
+    for block in model.layers:
+        for name in ("in_proj", "out_proj"):
+            old = getattr(block.mixer, name)
+            setattr(block.mixer, name, LinearW4(torch.randn(old.out_features, old.in_features, device="cuda").bfloat16(), group_size=64))
+    del block, old
+    gc.collect()
+    assert all(ref() is not None for ref in read)  # and only then is the graph run again
+    with pytest.raises(RuntimeError, match="recreate"):
+        decoder.validate()
+    decoder.reset()
+    assert torch.equal(decoder(x), want)
