@@ -50,6 +50,38 @@ def _validate(value, forget, gate, state, reset) -> None:
             raise ValueError("the state must be float32")
 
 
+def _places_differ(t: torch.Tensor) -> bool:
+    """Whether the elements of a matrix lie in different places."""
+    if t.is_contiguous():
+        return True
+    (rows, columns), (down, right) = t.shape, t.stride()
+    if rows == 1 or columns == 1:
+        return (down if columns == 1 else right) > 0
+    common = math.gcd(down, right)
+    # i down = j right first happens at i = right / common, j = down / common
+    return down > 0 and right > 0 and (right // common >= rows or down // common >= columns)
+
+
+def _elementwise_safe(out: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether a kernel that reads each element of ``t`` before it writes the same one of ``out``, in any order of
+    elements, is right: they are one view, or they share no place (as far as the strides show it)."""
+    if out is t:
+        return True
+    apart = out.data_ptr() - t.data_ptr()
+    if out.dtype == t.dtype and out.stride() == t.stride():
+        if apart == 0:
+            return True
+        (rows, columns), (down, right) = out.shape, out.stride()
+        if right == 1 and down >= columns and apart % out.element_size() == 0:  # rows of one matrix, two parts of it perhaps
+            i, j = divmod(apart // out.element_size(), down)
+            return not (abs(i) < rows and j < columns or abs(i + 1) < rows and down - j < columns)
+
+    def bytes_(m):
+        return (sum((n - 1) * s for n, s in zip(m.shape, m.stride())) + 1) * m.element_size()
+
+    return apart >= bytes_(t) or -apart >= bytes_(out)
+
+
 def _scan_torch(value, forget, gate, state, reset):
     """Differentiable form in (at least) float32: neighbours at distances 1, 2, 4, ... joined."""
     wide = torch.promote_types(value.dtype, torch.float32)
@@ -126,8 +158,8 @@ def gated_step(value: torch.Tensor, forget: torch.Tensor, state: torch.Tensor, g
                out_state: torch.Tensor | None = None):
     """One token: ``(y [B, C], new state [B, C] float32)`` from ``value``, ``forget``, ``gate``
     ``[B, C]`` and the float32 ``state``. ``out_state`` receives the new state and may be ``state``
-    itself (in-place decoding). Not differentiable on CUDA: sequences under autograd take
-    :func:`gated_scan`."""
+    itself (in-place decoding) or share memory with it in another way, but its elements lie in places of
+    their own. Not differentiable on CUDA: sequences under autograd take :func:`gated_scan`."""
     if value.dim() != 2:
         raise ValueError("value must have shape [B, C]")
     if state is None:
@@ -141,6 +173,8 @@ def gated_step(value: torch.Tensor, forget: torch.Tensor, state: torch.Tensor, g
         raise ValueError("gated step tensors must be on the same device")
     if out_state is not None and (out_state.shape != shape or out_state.dtype != torch.float32 or out_state.device != device):
         raise ValueError("out_state must be float32 and match the state's shape and device")
+    if out_state is not None and not _places_differ(out_state):
+        raise ValueError("out_state has several elements in one place")
     if not value.is_cuda or value.numel() == 0:
         if value.numel() == 0:
             y, new = value.clone(), state.clone()
@@ -156,9 +190,14 @@ def gated_step(value: torch.Tensor, forget: torch.Tensor, state: torch.Tensor, g
                                     or (gate is not None and gate.requires_grad)):
         raise ValueError("gated_step does not support gradients on CUDA; use gated_scan")
     y = torch.empty(shape[0], shape[1], device=device, dtype=dtype)  # plain ints: half the time of a torch.Size
-    new = torch.empty_like(state) if out_state is None else out_state
+    new = out_state
+    # threads take the elements in any order: what one still has to read must not be written by another
+    if out_state is None or ((out_state is not state or dtype == torch.float32)
+                             and not all(_elementwise_safe(out_state, t) for t in (state, value, forget, gate)
+                                         if t is not None and t.dtype == torch.float32)):
+        new = torch.empty(shape[0], shape[1], device=device, dtype=torch.float32)
     _ext.gated_step(value, forget, gate, state, y=y, out_state=new)
-    return y, new
+    return y, new if new is out_state or out_state is None else out_state.copy_(new)
 
 
 class _GatedMixer(nn.Module):

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from _operator_refs import gated_scan64
-from mamba3_b200 import GatedRecurrence, gated_scan, gated_step
+from mamba3_b200 import GatedRecurrence, gated_scan, gated_step, recurrence
 
 
 def _inputs(batch, length, channels, dtype=torch.float64, gate=True, seed=0):
@@ -108,3 +108,62 @@ def test_module_refusals():
         model.step(torch.randn(2, 2, 8))
     with pytest.raises(ValueError, match="cache for 1 layers"):
         model.step(torch.randn(2, 1, 8), [])
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (1, 4), (4, 1), (2, 3), (3, 2), (4, 5)])
+def test_places_and_shared_memory_by_enumeration(shape):
+    """Every pair of strides up to 6 and every distance up to 30 elements, against the sets of places."""
+    buffer = torch.zeros(200)
+    places = torch.arange(200)
+    for down in range(7):
+        for right in range(7):
+            t = buffer.as_strided(shape, (down, right), 60)
+            mine = places.as_strided(shape, (down, right), 60).flatten().tolist()
+            assert recurrence._places_differ(t) == (len(set(mine)) == len(mine))
+            for apart in range(-30, 31):
+                other = places.as_strided(shape, (down, right), 60 + apart).flatten().tolist()
+                safe = recurrence._elementwise_safe(buffer.as_strided(shape, (down, right), 60 + apart), t)
+                shared = not set(other).isdisjoint(mine)
+                assert not (safe and shared) or apart == 0
+                if right == 1 and down >= shape[1]:  # rows of a matrix: never taken for shared when they are not
+                    assert safe == (not shared) or apart == 0
+
+
+def _out_states(state):
+    """Destinations in the state's own memory: the state, shifted by an element and by a row, beside it, transposed."""
+    rows, columns = state.shape
+    for down, offset in ((columns, 0), (columns, 1), (columns, columns), (2 * columns, columns), (2 * columns, columns - 1)):
+        buffer = torch.zeros((rows + 2) * 2 * columns, device=state.device)
+        held = buffer.as_strided(state.shape, (down, 1))
+        held.copy_(state)
+        yield held, buffer.as_strided(state.shape, (down, 1), offset)
+    square = state[:, :rows].contiguous()
+    yield square, square.t()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_step_into_memory_shared_with_the_state(device):
+    g = torch.Generator().manual_seed(0)
+    value, forget, gate, state = (torch.randn(33, 600, generator=g).to(device) for _ in range(4))
+    for held, out in _out_states(state):
+        columns = held.shape[1]
+        want_y, want = gated_step(value[:, :columns], forget[:, :columns], held.clone(), gate[:, :columns])
+        y, new = gated_step(value[:, :columns], forget[:, :columns], held, gate[:, :columns], out_state=out)
+        assert new is out and torch.equal(out, want) and torch.equal(y, want_y)
+    # activations in the destination's memory
+    buffer = torch.zeros(34, 600, device=device)
+    buffer[1:] = value
+    want_y, want = gated_step(value, forget, state)
+    y, new = gated_step(buffer[1:], forget, state, out_state=buffer[:-1])
+    assert torch.equal(new, want) and torch.equal(y, want_y)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_step_refuses_a_destination_of_shared_places(device):
+    v, state = torch.randn(4, 6, device=device), torch.zeros(4, 6, device=device)
+    buffer = torch.zeros(40, device=device)
+    for out in (buffer[:6].expand(4, 6), buffer.as_strided((4, 6), (5, 1)), buffer.as_strided((4, 6), (1, 2))):
+        with pytest.raises(ValueError, match="several elements"):
+            gated_step(v, v, state, out_state=out)
+        with pytest.raises(ValueError, match="several elements"):
+            gated_step(v, v, out, out_state=out)
