@@ -696,7 +696,7 @@ bool pairs_written(const m3_tensor& t, const m3_gated_args& a, int elem) {
 bool encode(CUtensorMap* map, const m3_tensor& t, const m3_gated_args& a, int elem) {
   const PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
   if (enc == nullptr) return false;
-  const int64_t row = (int64_t)(a.channels * elem + 15) / 16 * 16;  // a stride that is never used
+  const int64_t row = ((int64_t)a.channels * elem + 15) / 16 * 16;  // a stride that is never used
   const int64_t token = a.length == 1 ? row : t.stride[1] * elem;
   const cuuint64_t dims[3] = {(cuuint64_t)a.channels, (cuuint64_t)a.length, (cuuint64_t)a.batch};
   const cuuint64_t strides[2] = {(cuuint64_t)token, (cuuint64_t)(a.batch == 1 ? row : t.stride[0] * elem)};
@@ -790,6 +790,8 @@ bool shaped(const m3_tensor& t, int ndim, int dtype) { return t.data == nullptr 
 int check(const m3_gated_args& a, bool backward) {
   if (a.batch <= 0 || a.length <= 0 || a.channels <= 0)
     return report_error(M3_ERR_SHAPE, "gated scan: batch, length and channels must be positive");
+  constexpr int32_t kMost = INT32_MAX - 4096;  // channels past the last block's still count in 32 bits
+  if (a.channels > kMost) return report_error(M3_ERR_SHAPE, "gated scan: channels above 2^31 - 4097");
   if (a.batch > 65535) return report_error(M3_ERR_SHAPE, "gated scan: batch above 65535");
   if (!a.value.data || !a.forget.data) return report_error(M3_ERR_ARGUMENT, "gated scan: value and forget are required");
   const int act = a.value.dtype;

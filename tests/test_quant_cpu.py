@@ -156,3 +156,13 @@ def test_c_entries_reject_malformed_arguments_without_a_device():
     assert lib.m3_orthogonalize(_ext._ORTH_FORMAT.pack(4, 4, 1, 65, -1, 1, 1, 1, *absent * 3), None) == 4
     assert lib.m3_orthogonalize(_ext._ORTH_FORMAT.pack(4, 4, 1, 5, -1, 1, 1, 1, *absent * 3), None) == 4
     assert lib.m3_orthogonalize_workspace_bytes(_ext._ORTH_FORMAT.pack(0, 4, 1, 5, -1, 1, 1, 1, *absent * 3)) == -1
+
+
+def test_gated_entries_reject_widths_that_overflow():
+    """Channels past the last block's are counted in 32 bits by the kernels: such widths end before a launch."""
+    lib, absent = _ext.load(), _ext._ABSENT
+    for length in (1, 4):
+        for channels in (2 ** 31 - 1, 2 ** 31 - 4096):
+            assert lib.m3_gated_scan_fwd(_ext._GATED_FORMAT.pack(length, 1, channels, -1, 0, *absent * 14), None) == 1
+            assert lib.m3_gated_scan_bwd(_ext._GATED_FORMAT.pack(length, 1, channels, -1, 0, *absent * 14), None) == 1
+    assert lib.m3_gated_scan_fwd(_ext._GATED_FORMAT.pack(1, 1, 2 ** 31 - 4097, -1, 0, *absent * 14), None) == 4
