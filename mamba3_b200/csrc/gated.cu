@@ -118,6 +118,9 @@ template <> struct Two<__nv_bfloat16> {
   static __device__ __forceinline__ __nv_bfloat162 close(float2 v) { return __float22bfloat162_rn(v); }
 };
 
+// A block's sequence: sequences lie along the grid's y, and its z where they are more than y may have.
+__device__ __forceinline__ int sequence() { return blockIdx.z * gridDim.y + blockIdx.y; }
+
 // ---- tiles ---------------------------------------------------------------------------------------
 
 // Tokens t0 .. t0 + 63 of channels c0 .. c0 + 63 to a tile [64][64], for inputs that TMA cannot read: any
@@ -384,7 +387,8 @@ __global__ void __launch_bounds__(kFwdThreads, 4)
   float2* next = reinterpret_cast<float2*>(peers + (cluster > 1 ? 2 * cluster * 32 : 0));  // the state after the tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = cluster > 1 ? cluster_rank() : 0;
-  const int b = blockIdx.y, c0 = blockIdx.x / cluster * kChannels, c = c0 + 2 * lane;
+  const int b = sequence(), c0 = blockIdx.x / cluster * kChannels, c = c0 + 2 * lane;
+  if (b >= a.batch) return;  // as the whole cluster does
   Pipeline<T, kTensors, kFwdThreads, kVec> pipe;
   pipe.ntiles = (a.length + kTile - 1) / kTile;
   pipe.groups = (pipe.ntiles + cluster - 1) / cluster;
@@ -479,7 +483,8 @@ __global__ void __launch_bounds__(kBwdThreads, 2)
   float2* next = reinterpret_cast<float2*>(peers + (cluster > 1 ? 2 * cluster * 32 : 0));  // In before the tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = cluster > 1 ? cluster_rank() : 0;
-  const int b = blockIdx.y, c0 = blockIdx.x / cluster * kChannels, c = c0 + 2 * lane;
+  const int b = sequence(), c0 = blockIdx.x / cluster * kChannels, c = c0 + 2 * lane;
+  if (b >= a.batch) return;  // as the whole cluster does
   Pipeline<T, kTensors, kBwdThreads, kVec> pipe;
   pipe.ntiles = (a.length + kTile - 1) / kTile;
   pipe.groups = (pipe.ntiles + cluster - 1) / cluster;
@@ -609,8 +614,8 @@ __global__ void __launch_bounds__(kBwdThreads, 2)
 // (76 % of a copy), 1 x 5120 1.4 in a graph: a launch, and the latency of one load.
 template <typename T, int kWide>
 __global__ void __launch_bounds__(128) gated_step_kernel(const m3_gated_args a) {
-  const int c = (blockIdx.x * 128 + threadIdx.x) * kWide, b = blockIdx.y;
-  if (c >= a.channels) return;
+  const int c = (blockIdx.x * 128 + threadIdx.x) * kWide, b = sequence();
+  if (c >= a.channels || b >= a.batch) return;
   auto at = [&](const m3_tensor& t) { return static_cast<T*>(t.data) + b * t.stride[0] + c * t.stride[2]; };
   float h[kWide], f[kWide], v[kWide], q[kWide], y[kWide];
   auto get = [&](const T* p, float* to) {
@@ -660,6 +665,12 @@ __global__ void __launch_bounds__(128) gated_step_kernel(const m3_gated_args a) 
 
 // ---- host ----------------------------------------------------------------------------------------
 
+// A grid of `blocks` for each sequence; see sequence().
+dim3 sequences_grid(int64_t blocks, int batch) {
+  const int z = (batch + 65534) / 65535;
+  return dim3((unsigned)blocks, (unsigned)((batch + z - 1) / z), (unsigned)z);
+}
+
 // Rows of `bytes`-aligned runs of channels: unit stride, aligned start and aligned batch and token strides.
 bool rows_aligned(const m3_tensor& t, int elem, int bytes) {
   return t.data == nullptr || (t.stride[2] == 1 && reinterpret_cast<uintptr_t>(t.data) % bytes == 0 &&
@@ -675,7 +686,7 @@ template <typename T> cudaError_t launch_step_token(const m3_gated_args& a, cuda
                     rows_aligned(a.gate, kElem, 4 * kElem) && rows_aligned(a.y, kElem, 4 * kElem) && state_aligned(a.state) &&
                     state_aligned(a.out_state);
   const int per_block = 128 * (wide ? 4 : 1);
-  const dim3 grid((unsigned)((a.channels + per_block - 1) / per_block), (unsigned)a.batch);
+  const dim3 grid = sequences_grid((a.channels + per_block - 1) / per_block, a.batch);
   if (wide) gated_step_kernel<T, 4><<<grid, 128, 0, stream>>>(a);
   else gated_step_kernel<T, 1><<<grid, 128, 0, stream>>>(a);
   return cudaGetLastError();
@@ -740,7 +751,7 @@ cudaError_t launch_tiles(K kernel, const m3_gated_args& a, const Maps& maps, int
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a.channels + kChannels - 1) / kChannels * cluster), (unsigned)a.batch);
+  cfg.gridDim = sequences_grid((int64_t)(a.channels + kChannels - 1) / kChannels * cluster, a.batch);
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -792,7 +803,7 @@ int check(const m3_gated_args& a, bool backward) {
     return report_error(M3_ERR_SHAPE, "gated scan: batch, length and channels must be positive");
   constexpr int32_t kMost = INT32_MAX - 4096;  // channels past the last block's still count in 32 bits
   if (a.channels > kMost) return report_error(M3_ERR_SHAPE, "gated scan: channels above 2^31 - 4097");
-  if (a.batch > 65535) return report_error(M3_ERR_SHAPE, "gated scan: batch above 65535");
+  if (a.batch > INT32_MAX - 65536) return report_error(M3_ERR_SHAPE, "gated scan: batch above 2^31 - 65537");
   if (!a.value.data || !a.forget.data) return report_error(M3_ERR_ARGUMENT, "gated scan: value and forget are required");
   const int act = a.value.dtype;
   if (act != M3_F32 && act != M3_F16 && act != M3_BF16)

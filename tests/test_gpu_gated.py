@@ -310,3 +310,26 @@ def test_threads_with_different_shapes():
     for t in threads:
         t.join()
     assert not failed
+
+
+@pytest.mark.parametrize("length", [1, 3, 70])
+@pytest.mark.parametrize("channels", [2, 8])
+def test_more_sequences_than_a_grid_dimension(length, channels):
+    """65,535 blocks go along a grid's y; the sequences past them and the last ones, which a rounded-up grid has too."""
+    batch = 2 * 65535 + 5
+    value, forget, gate, state, reset = _inputs(batch, length, channels, torch.bfloat16)
+    y, final = gated_scan(value, forget, gate, initial_state=state, reset=reset)
+    want_y, want_final = gated_scan64(value, forget, gate, state, reset)
+    assert_rounded(y, want_y, SUMS)
+    assert_rounded(final, want_final, SUMS)
+    dy, dstate = torch.randn_like(value), torch.randn_like(state)
+    got = _gradients(value, forget, gate, state, reset, dy, dstate,
+                     lambda v, f, q, s, r: gated_scan(v, f, q, initial_state=s, reset=r))
+    want = _gradients(value.double(), forget.double(), gate.double(), state.double(), reset, dy, dstate, gated_scan64)
+    for a, e in zip(got, want):
+        assert_rounded(a, e, 2 * SUMS)
+    if length == 1:
+        y, new = gated_step(value[:, 0], forget[:, 0], state, gate[:, 0])
+        want_y, want = gated_scan64(value, forget, gate, state)
+        assert_rounded(y, want_y[:, 0], SUMS)
+        assert_rounded(new, want, SUMS)
