@@ -198,6 +198,7 @@ typedef struct m3_gated_args {
 } m3_gated_args;
 
 int m3_gated_tile(void);
+int m3_gated_cluster(const m3_gated_args* args, int backward); /* CTAs that a call lets share a sequence; launches nothing */
 int m3_gated_scan_fwd(const m3_gated_args* args, void* stream);
 int m3_gated_scan_bwd(const m3_gated_args* args, void* stream);
 

@@ -165,6 +165,8 @@ def load() -> ctypes.CDLL:
         lib.m3_ssd_train_bwd.restype = ctypes.c_int
         lib.m3_gated_tile.argtypes = []
         lib.m3_gated_tile.restype = ctypes.c_int
+        lib.m3_gated_cluster.argtypes = [ctypes.c_char_p, ctypes.c_int]
+        lib.m3_gated_cluster.restype = ctypes.c_int
         for name in ("m3_gated_scan_fwd", "m3_gated_scan_bwd", "m3_linear_w4", "m3_orthogonalize"):
             getattr(lib, name).argtypes = [ctypes.c_char_p, ctypes.c_void_p]
             getattr(lib, name).restype = ctypes.c_int

@@ -12,6 +12,7 @@
 //   dforget_t = G_t (h_{t-1} - value_t) f_t (1 - f_t),   dgate_t = dy_t h_t silu'(gate_t),
 //   dstate_0  = In_0.
 #include <algorithm>
+#include <atomic>
 #include <string>
 #include <type_traits>
 
@@ -719,9 +720,62 @@ bool encode(CUtensorMap* map, const m3_tensor& t, const m3_gated_args& a, int el
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename K>
-cudaError_t launch_tiles(K kernel, const m3_gated_args& a, const Maps& maps, int threads, int tile, int tensors, int run_maps,
-                         cudaStream_t stream) {
+template <typename T, bool kGate, bool kVec, bool kBackward> auto pass_kernel() {
+  if constexpr (kBackward) return gated_bwd_kernel<T, kGate, kVec>;
+  else return gated_fwd_kernel<T, kGate, kVec>;
+}
+
+// How a pass lies in a CTA.
+template <typename T, bool kGate, bool kBackward> struct Pass {
+  static constexpr int kThreads = kBackward ? kBwdThreads : kFwdThreads;
+  static constexpr int smem(int cluster) {
+    return smem_bytes(tile_bytes<T>(), (kBackward ? 3 : 2) + (kGate ? 1 : 0), kBackward ? 2 * kBwdWarps : kFwdWarps, cluster);
+  }
+  // CTAs of a cluster of `size` that an SM has room for: by shared memory, which grows with the cluster, and by registers
+  // at the 128 that both kernels take.
+  static constexpr int room(int size) { return std::min(227 * 1024 / (smem(size) + 1024), 65536 / (128 * kThreads)); }
+
+  static cudaLaunchConfig_t config(dim3 grid, int cluster, cudaLaunchAttribute* attr, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem(cluster);
+    cfg.stream = stream;
+    attr->id = cudaLaunchAttributeClusterDimension;
+    attr->val.clusterDim.x = cluster;
+    attr->val.clusterDim.y = attr->val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    return cfg;
+  }
+  // The limits are the kernel's, not the launch's: the largest cluster's always, or another thread with a shorter sequence
+  // could lower them between this call and a launch.
+  template <typename K> static cudaError_t raise_limits(K kernel) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem(kMaxCluster));
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  }
+  // Clusters of 16 that the device hosts at once where an SM has room for one of their CTAs only; 0 without a device.
+  static int hosted() {
+    static std::atomic<int> cached[64];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+      cudaGetLastError();
+      return 0;
+    }
+    if (const int held = cached[dev].load(std::memory_order_relaxed)) return held - 1;
+    const auto kernel = pass_kernel<T, kGate, true, kBackward>();
+    cudaLaunchAttribute attr[1];
+    const cudaLaunchConfig_t cfg = config(dim3(kMaxCluster), kMaxCluster, attr, nullptr);
+    if (raise_limits(kernel) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      return 0;
+    }
+    cached[dev].store(n + 1, std::memory_order_relaxed);
+    return n;
+  }
+};
+
+template <typename P> int cluster_size(const m3_gated_args& a) {
   const int64_t ntiles = (a.length + kTile - 1) / kTile;
   const int64_t blocks = (int64_t)a.batch * ((a.channels + kChannels - 1) / kChannels);
   // A cluster takes a sequence's tiles together while its CTAs still have room on the GPU at once: clusters of up to
@@ -729,59 +783,46 @@ cudaError_t launch_tiles(K kernel, const m3_gated_args& a, const Maps& maps, int
   // as a tile, up to two CTAs an SM (1 x 65536 x 1536: 308 us in eights, 328 in sixteens; 1 x 32768 x 128: 83 us in
   // sixteens, 136 in eights), and tens where sixteens have no such room (1 x 65536 x 1536: 267 us, backward 647 against
   // 762). Where the CTAs of eights have all their tiles under way from the start, they take all the room too
-  // (3 x 777 x 1001: 17 us, 26 in fours). Past 8 CTAs, a cluster's size without conditions, only where two fit an SM.
-  // (CTAs that an SM has room for: by shared memory, and by registers at the 128 that both kernels take)
-  const int per_sm = std::min(227 * 1024 / (smem_bytes(tile, tensors, run_maps, 2) + 1024), 65536 / (128 * threads));
-  const int most = per_sm > 1 ? kMaxCluster : 8;
+  // (3 x 777 x 1001: 17 us, 26 in fours). Past 8 CTAs, a cluster's size without conditions, only where two fit an SM; or
+  // sixteens where the device has SMs enough side by side for all of them (float32 with a gate, whose sixteens fit one
+  // an SM: 1 x 32768 x 128 in 80 us, 117 in tens; 1 x 65536 x 1024, 16 clusters that it has not: 438 us, 295 in tens).
   int cluster = 1;
-  while (cluster < most && 2 * cluster <= ntiles) {
-    const bool all_room = cluster < 4 || (cluster == 4 && 8 * kStages >= ntiles);
-    if (2 * cluster * blocks > (int64_t)sm_count() * (all_room ? per_sm : std::min(per_sm, 2))) break;
-    cluster *= 2;
+  for (int size = 2; size <= kMaxCluster && size <= ntiles; size *= 2) {
+    const bool all_room = size < 8 || (size == 8 && 8 * kStages >= ntiles);
+    if (size * blocks > (int64_t)sm_count() * (all_room ? P::room(size) : std::min(P::room(size), 2))) break;
+    if (size > 8 && P::room(size) < 2 && blocks > P::hosted()) break;
+    cluster = size;
   }
-  if (cluster == 8 && most > 8 && 10 <= ntiles && 10 * blocks <= 2 * (int64_t)sm_count()) cluster = 10;
-  const int smem = smem_bytes(tile, tensors, run_maps, cluster);
-  // The limit is the kernel's, not the launch's: the largest cluster's always, or another thread with a shorter sequence
-  // could lower it between this call and the launch below.
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       smem_bytes(tile, tensors, run_maps, kMaxCluster));
+  if (cluster == 8 && P::room(10) >= 2 && 10 <= ntiles && 10 * blocks <= 2 * (int64_t)sm_count()) cluster = 10;
+  return cluster;
+}
+
+template <typename T, bool kGate, bool kBackward> cudaError_t launch_tiles(const m3_gated_args& a, const Maps& maps, bool vec, cudaStream_t stream) {
+  using P = Pass<T, kGate, kBackward>;
+  const int cluster = cluster_size<P>(a);
+  const auto kernel = vec ? pass_kernel<T, kGate, true, kBackward>() : pass_kernel<T, kGate, false, kBackward>();
+  const cudaError_t e = P::raise_limits(kernel);
   if (e != cudaSuccess) return e;
-  if (cluster > 8) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = sequences_grid((int64_t)(a.channels + kChannels - 1) / kChannels * cluster, a.batch);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  const dim3 grid = sequences_grid((int64_t)(a.channels + kChannels - 1) / kChannels * cluster, a.batch);
+  const cudaLaunchConfig_t cfg = P::config(grid, cluster, attr, stream);
   return cudaLaunchKernelEx(&cfg, kernel, maps, a, cluster);
 }
 
 template <typename T> cudaError_t launch_fwd(const m3_gated_args& a, cudaStream_t stream) {
   if (a.length == 1) return launch_step_token<T>(a, stream);
-  constexpr int kElem = sizeof(T), tile = tile_bytes<T>();
+  constexpr int kElem = sizeof(T);
   Maps maps = {};
   const bool vec = tma_reads(a.forget, a, kElem) && tma_reads(a.value, a, kElem) && tma_reads(a.gate, a, kElem) &&
                    pairs_written(a.y, a, kElem);
   if (vec && !(encode(&maps.map[0], a.forget, a, kElem) && encode(&maps.map[1], a.value, a, kElem) &&
                (a.gate.data == nullptr || encode(&maps.map[2], a.gate, a, kElem))))
     return cudaErrorInvalidValue;
-  if (a.gate.data)
-    return launch_tiles(vec ? gated_fwd_kernel<T, true, true> : gated_fwd_kernel<T, true, false>, a, maps, kFwdThreads, tile, 3,
-                        kFwdWarps, stream);
-  return launch_tiles(vec ? gated_fwd_kernel<T, false, true> : gated_fwd_kernel<T, false, false>, a, maps, kFwdThreads, tile, 2,
-                      kFwdWarps, stream);
+  return a.gate.data ? launch_tiles<T, true, false>(a, maps, vec, stream) : launch_tiles<T, false, false>(a, maps, vec, stream);
 }
 
 template <typename T> cudaError_t launch_bwd(const m3_gated_args& a, cudaStream_t stream) {
-  constexpr int kElem = sizeof(T), tile = tile_bytes<T>();
+  constexpr int kElem = sizeof(T);
   Maps maps = {};
   const bool vec = tma_reads(a.forget, a, kElem) && tma_reads(a.value, a, kElem) && tma_reads(a.dy, a, kElem) &&
                    tma_reads(a.gate, a, kElem) && pairs_written(a.dvalue, a, kElem) && pairs_written(a.dforget, a, kElem) &&
@@ -789,11 +830,7 @@ template <typename T> cudaError_t launch_bwd(const m3_gated_args& a, cudaStream_
   if (vec && !(encode(&maps.map[0], a.forget, a, kElem) && encode(&maps.map[1], a.value, a, kElem) &&
                encode(&maps.map[2], a.dy, a, kElem) && (a.gate.data == nullptr || encode(&maps.map[3], a.gate, a, kElem))))
     return cudaErrorInvalidValue;
-  if (a.gate.data)
-    return launch_tiles(vec ? gated_bwd_kernel<T, true, true> : gated_bwd_kernel<T, true, false>, a, maps, kBwdThreads, tile, 4,
-                        2 * kBwdWarps, stream);
-  return launch_tiles(vec ? gated_bwd_kernel<T, false, true> : gated_bwd_kernel<T, false, false>, a, maps, kBwdThreads, tile, 3,
-                      2 * kBwdWarps, stream);
+  return a.gate.data ? launch_tiles<T, true, true>(a, maps, vec, stream) : launch_tiles<T, false, true>(a, maps, vec, stream);
 }
 
 bool shaped(const m3_tensor& t, int ndim, int dtype) { return t.data == nullptr || (t.ndim == ndim && t.dtype == dtype); }
@@ -835,6 +872,18 @@ int launched(const char* what, cudaError_t e) {
 }  // namespace m3
 
 extern "C" int m3_gated_tile(void) { return m3::kTile; }
+
+extern "C" int m3_gated_cluster(const m3_gated_args* args, int backward) {
+  using namespace m3;
+  if (args == nullptr || args->batch <= 0 || args->length <= 0 || args->channels <= 0) return 0;
+  if (args->length == 1 && !backward) return 1;
+  auto of = [&](auto type) {  // 16-bit types lie alike
+    using T = decltype(type);
+    if (args->gate.data) return backward ? cluster_size<Pass<T, true, true>>(*args) : cluster_size<Pass<T, true, false>>(*args);
+    return backward ? cluster_size<Pass<T, false, true>>(*args) : cluster_size<Pass<T, false, false>>(*args);
+  };
+  return args->value.dtype == M3_F32 ? of(0.0f) : of(__half());
+}
 
 extern "C" int m3_gated_scan_fwd(const m3_gated_args* args, void* stream) {
   using namespace m3;

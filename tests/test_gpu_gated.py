@@ -333,3 +333,24 @@ def test_more_sequences_than_a_grid_dimension(length, channels):
         want_y, want = gated_scan64(value, forget, gate, state)
         assert_rounded(y, want_y[:, 0], SUMS)
         assert_rounded(new, want, SUMS)
+
+
+@pytest.mark.parametrize("length", [650, 1300])
+@pytest.mark.parametrize("channels", [128, 1216, 1300, 2368, 4736])
+@pytest.mark.parametrize("gated", [True, False])
+def test_every_split_of_a_float32_sequence(length, channels, gated):
+    """Tiles of float32 leave room for fewer CTAs of a cluster, with a gate for fewer still."""
+    value, forget, gate, state, reset = _inputs(1, length, channels, torch.float32, gate=gated, seed=channels)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    dy = torch.randn(1, length, channels, device="cuda", generator=g)
+    dstate = torch.randn(1, channels, device="cuda", generator=g)
+    run = lambda v, f, q, s, r: gated_scan(v, f, q, initial_state=s, reset=r)  # noqa: E731
+    y, final = run(value, forget, gate, state, reset)
+    want_y, want_final = gated_scan64(value, forget, gate, state, reset)
+    assert_rounded(y, want_y, SUMS)
+    assert_rounded(final, want_final, SUMS)
+    got = _gradients(value, forget, gate, state, reset, dy, dstate, run)
+    want = _gradients(value.double(), forget.double(), None if gate is None else gate.double(), state.double(), reset, dy, dstate,
+                      gated_scan64)
+    for i, (a, e) in enumerate(zip(got, want)):
+        assert_rounded(a, e, 2 * SUMS, f"gradient {i}")

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from _operator_refs import gated_scan64
-from mamba3_b200 import GatedRecurrence, gated_scan, gated_step, recurrence
+from mamba3_b200 import GatedRecurrence, _ext, gated_scan, gated_step, recurrence
 
 
 def _inputs(batch, length, channels, dtype=torch.float64, gate=True, seed=0):
@@ -167,3 +167,28 @@ def test_step_refuses_a_destination_of_shared_places(device):
             gated_step(v, v, state, out_state=out)
         with pytest.raises(ValueError, match="several elements"):
             gated_step(v, v, out, out_state=out)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("backward", [False, True])
+def test_clusters_have_room(dtype, gate, backward):
+    """Past 8 CTAs, which any GPU hosts, only where two of a cluster's CTAs fit an SM (227 KB, 1 KB of it a block's own,
+    and 64 K registers) or, with a device to ask, where it hosts all clusters at once; and no more CTAs than there is
+    room for on 148 SMs."""
+    lib, size = _ext.load(), torch.empty((), dtype=dtype).element_size()
+    threads, tensors, maps = (256, 4 if gate else 3, 16) if backward else (128, 3 if gate else 2, 4)
+    sizes = set()
+    for length in (2, 64, 129, 300, 640, 1024, 4096, 65536):
+        for batch, channels in ((1, 64), (1, 128), (1, 640), (1, 1024), (2, 1000), (1, 1800), (3, 1001), (8, 2048), (70000, 3)):
+            tensor = (1 << 20, _ext._TENSOR_CODES[dtype] | 3 << 32, 0, 0, 0, 0, 0, 0)
+            args = _ext._GATED_FORMAT.pack(length, batch, channels, -1, 0, *tensor, *tensor, *(tensor if gate else _ext._ABSENT),
+                                           *_ext._ABSENT * 11)
+            cluster = lib.m3_gated_cluster(args, backward)
+            memory = 2 * tensors * 64 * 64 * size + (maps + 2 * cluster) * 512 + 512 + 1024
+            room = min(227 * 1024 // memory, 65536 // (128 * threads))
+            assert cluster == 1 or cluster <= -(-length // 64)
+            assert cluster <= 8 or room >= 2 or (torch.cuda.is_available() and cluster == 16)
+            assert cluster == 1 or cluster * batch * -(-channels // 64) <= 148 * room
+            sizes.add(cluster)
+    assert sizes >= {1, 2, 4, 8}
