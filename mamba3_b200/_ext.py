@@ -14,6 +14,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 _LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libmamba3_b200.so"
 
@@ -496,6 +497,13 @@ def gemv(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     args.x, args.w, args.y = _desc(x2), _desc(w), _desc(y)
     _check(lib.m3_gemv(ctypes.byref(args), ctypes.c_void_p(torch.cuda.current_stream(x.device).cuda_stream)), lib)
     return y.view(*x.shape[:-1], w.shape[0])
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether a tensor carries a tangent of ``torch.autograd.forward_ad``. Such a dual tensor has ``requires_grad``
+    False and data like any other's; a kernel that runs on it gives a result without a tangent, a derivative of 0."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                                  for t in tensors)
 
 
 # ---- operators whose argument structs are packed in one go -----------------------------------------

@@ -45,7 +45,7 @@ def _default_chunk_sizes(mimo_rank: int) -> tuple[int, int]:
 
 def _few_rows(hidden: torch.Tensor, weight: torch.Tensor) -> bool:
     """Decode-step projections (at most 4 rows, inference) run as a weight stream on m3_gemv."""
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad) or _ext.has_tangent(hidden, weight):
         return False
     return _ext.gemv_eligible(hidden, weight)
 

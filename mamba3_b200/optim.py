@@ -48,6 +48,8 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, *, coefficients=COEFFICI
         return update.to(out_dtype)
     if not update.is_cuda:
         return _orthogonalize_torch(update, steps, coefficients).to(out_dtype).contiguous()
+    if _ext.has_tangent(update):
+        raise ValueError("orthogonalize has no forward-mode derivative on CUDA")
     if update.dtype not in _FLOATS or out_dtype not in _FLOATS:
         raise TypeError(f"unsupported dtypes {update.dtype} -> {out_dtype}")
     stack = update.unsqueeze(0) if update.dim() == 2 else update.flatten(0, -3)

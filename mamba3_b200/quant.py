@@ -102,6 +102,8 @@ def linear_w4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros:
         return F.linear(x.float(), dequantize_w4(codes, scales, zeros, x.shape[-1], group_size=group_size)).to(x.dtype)
     if x.dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"linear_w4 needs float16 or bfloat16 activations on CUDA, got {x.dtype}")
+    if _ext.has_tangent(x, scales, zeros):
+        raise ValueError("linear_w4 is inference only: it has no forward-mode derivative on CUDA")
     if scales.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise TypeError(f"unsupported scale dtype {scales.dtype}")
     if x.dim() == 2:

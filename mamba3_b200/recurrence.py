@@ -131,6 +131,7 @@ def gated_scan(value: torch.Tensor, forget: torch.Tensor, gate: torch.Tensor | N
 
     ``value``, ``forget`` (logits) and the optional output ``gate`` are ``[B, L, C]`` of one dtype
     (float32, float16 or bfloat16), of any strides: columns of one projection are read in place.
+    On CUDA it has gradients in reverse mode, once; forward mode is refused.
     ``initial_state`` is ``[B, C]`` float32 (zeros without it). ``reset`` ``[B, L]`` (bool) marks
     tokens that start a document: they see a zero state. The state is held in float32; ``y`` and the
     gradients are rounded once, to the inputs' dtype.
@@ -144,6 +145,8 @@ def gated_scan(value: torch.Tensor, forget: torch.Tensor, gate: torch.Tensor | N
         return value.clone(), state
     if not value.is_cuda:
         return _scan_torch(value, forget, gate, initial_state, reset)
+    if _ext.has_tangent(value, forget, gate, initial_state):
+        raise ValueError("gated_scan has no forward-mode derivative on CUDA")
     if torch.is_grad_enabled() and (value.requires_grad or forget.requires_grad
                                     or (gate is not None and gate.requires_grad)
                                     or (initial_state is not None and initial_state.requires_grad)):
@@ -190,6 +193,8 @@ def gated_step(value: torch.Tensor, forget: torch.Tensor, state: torch.Tensor, g
                                     or (gate is not None and gate.requires_grad)):
         raise ValueError("gated_step does not support gradients on CUDA; use gated_scan")
     y = torch.empty(shape[0], shape[1], device=device, dtype=dtype)  # plain ints: half the time of a torch.Size
+    if _ext.has_tangent(value, forget, gate, state):
+        raise ValueError("gated_step has no forward-mode derivative on CUDA")
     new = out_state
     # threads take the elements in any order: what one still has to read must not be written by another
     if out_state is None or ((out_state is not state or dtype == torch.float32)
