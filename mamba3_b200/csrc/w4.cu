@@ -11,7 +11,9 @@
 // threads share an output row, and of every group a thread has group / 4 neighbouring columns, one load of 4, 8 or
 // 16 bytes. Products of 16-bit values by code - 8 are exact, sums float32, scaled group by group:
 //   y = sum_g s (sum x (q - 8) - (z - 8) sum x),
-// the sums of x by products with ones; y is rounded once.
+// the sums of x by products with ones; y is rounded once. That form loses two things: with an infinity in x it is inf - inf
+// where a code and its zero point are on one side of 8, and sum x (q - 8) can pass float32's range where s would bring it
+// back. Both leave a sum that is not finite, and such an output is taken again term by term, s (q - z) first.
 #include <algorithm>
 #include <string>
 #include <type_traits>
@@ -250,6 +252,28 @@ __host__ __device__ __forceinline__ bool x_in_units(const m3_w4_args& a) {
   return a.x.stride[1] == 1 && (a.rows == 1 || a.x.stride[0] % 8 == 0) && (reinterpret_cast<uintptr_t>(a.x.data) & 15) == 0;
 }
 
+// The definition of one output, for sums that are not finite. NaN ends it: nothing else follows from there.
+template <typename T> __device__ __noinline__ float by_definition(const m3_w4_args& a, int64_t row, int64_t out) {
+  const int type = a.scales.dtype, size = type == M3_F32 ? 4 : 2;
+  const T* x = static_cast<const T*>(a.x.data) + row * a.x.stride[0];
+  const uint8_t* codes = static_cast<const uint8_t*>(a.codes.data) + out * a.codes.stride[0];
+  auto at = [&](const m3_tensor& t, int64_t g) {
+    return widen(bits(static_cast<const uint8_t*>(t.data) + (out * t.stride[0] + g * t.stride[1]) * size, type), type);
+  };
+  float sum = 0.0f;
+  for (int64_t g = 0; g * a.group < a.in_dim && sum == sum; ++g) {
+    const float scale = at(a.scales, g), zero = a.zeros.data ? at(a.zeros, g) : 8.0f;
+    const int64_t first = g * a.group, last = min(a.in_dim, first + a.group);
+#pragma unroll 4
+    for (int64_t i = first; i < last; ++i) {
+      const int code = codes[(i >> 1) * a.codes.stride[1]] >> (i & 1 ? 4 : 0) & 15;
+      sum = fmaf(to_f(x[i * a.x.stride[1]]), scale * ((float)code - zero), sum);
+    }
+  }
+  return sum;
+}
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
+
 // ---- up to 8 rows --------------------------------------------------------------------------------
 // A stream of codes: one CTA for 16 outputs, its warps share the columns out, slab by slab, and meet in shared memory.
 // x, a few KB, comes from L1 as the products want it. 10768 x 2560, groups of 128: 6.3 us at one row (2.2 TB/s of codes),
@@ -259,7 +283,7 @@ __host__ __device__ __forceinline__ bool x_in_units(const m3_w4_args& a) {
 constexpr int kMostWarps = 16;
 
 template <typename T, int kWords, bool kFast, bool kZeros>
-__global__ void __launch_bounds__(32 * kMostWarps) w4_few_kernel(const m3_w4_args a) {
+__global__ void __launch_bounds__(32 * kMostWarps) w4_few_kernel(const __grid_constant__ m3_w4_args a) {
   using W = Weight<T, kWords, kFast, kZeros>;
   constexpr int kAhead = 2;  // slabs whose codes are under way
   __shared__ float part[kMostWarps][8][16];
@@ -346,6 +370,7 @@ __global__ void __launch_bounds__(32 * kMostWarps) w4_few_kernel(const m3_w4_arg
     if (r >= a.rows || out >= a.out_dim) continue;
     float v = 0.0f;
     for (int w = 0; w < warps; ++w) v += part[w][r][i & 15];
+    if (!finite(v)) v = by_definition<T>(a, r, out);
     yp[r * a.y.stride[0] + out * a.y.stride[1]] = from_f<T>(v);
   }
 }
@@ -443,8 +468,8 @@ __device__ __forceinline__ void load(uint32_t from, uint32_t (&r)[16]) {
 
 template <typename T, int kN, bool kZeros>
 __global__ void __launch_bounds__(Many<kN>::kThreads, 1)
-    w4_many_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_constant__ CUtensorMap x_map, const m3_w4_args a,
-                   int split, bool code_tiles, bool x_tiles) {
+    w4_many_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_constant__ CUtensorMap x_map,
+                   const __grid_constant__ m3_w4_args a, int split, bool code_tiles, bool x_tiles) {
   using M = Many<kN>;
   extern __shared__ uint8_t raw[];
   const uint32_t base = (umma::smem_u32(raw) + 1023u) & ~1023u;
@@ -748,9 +773,17 @@ __global__ void __launch_bounds__(Many<kN>::kThreads, 1)
   const int col0 = consumer ? M::kCols * ((warp - kProducers / 32 - 2) >> 2) : 0;
   if (split == 1) {
     if (consumer && o0 + out < a.out_dim) {
+      uint32_t again = 0;
 #pragma unroll
-      for (int n = 0; n < M::kCols; ++n)
-        if (col0 + n < rows) yp[(rows0 + col0 + n) * a.y.stride[0] + (o0 + out) * a.y.stride[1]] = from_f<T>(acc[n]);
+      for (int n = 0; n < M::kCols; ++n) {
+        if (col0 + n >= rows) continue;
+        yp[(rows0 + col0 + n) * a.y.stride[0] + (o0 + out) * a.y.stride[1]] = from_f<T>(acc[n]);
+        again |= finite(acc[n]) ? 0u : 1u << n;
+      }
+      for (; again; again &= again - 1) {
+        const int64_t row = rows0 + col0 + __ffs(again) - 1;
+        yp[row * a.y.stride[0] + (o0 + out) * a.y.stride[1]] = from_f<T>(by_definition<T>(a, row, o0 + out));
+      }
     }
     return;
   }
@@ -774,7 +807,9 @@ __global__ void __launch_bounds__(Many<kN>::kThreads, 1)
       asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(p) : "r"(at) : "memory");
       v += p;
     }
-    if (n < rows && o0 + oo < a.out_dim) yp[(rows0 + n) * a.y.stride[0] + (o0 + oo) * a.y.stride[1]] = from_f<T>(v);
+    if (n >= rows || o0 + oo >= a.out_dim) continue;
+    if (!finite(v)) v = by_definition<T>(a, rows0 + n, o0 + oo);
+    yp[(rows0 + n) * a.y.stride[0] + (o0 + oo) * a.y.stride[1]] = from_f<T>(v);
   }
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // no CTA leaves while another reads its sums

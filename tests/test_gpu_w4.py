@@ -209,3 +209,47 @@ def test_a_decoder_keeps_the_weights_that_its_graph_reads():
         decoder.validate()
     decoder.reset()
     assert torch.equal(decoder(x), want)
+
+
+def _check_nonfinite(x, codes, scales, zeros, group, y):
+    """Infinities with their signs and NaN where the definition has them; finite outputs within the bound."""
+    w = weight_w4(codes, scales, zeros, x.shape[-1], group)
+    want = torch.stack([(row * w).sum(1) for row in x.double()])  # term by term: nothing but the definition's products
+    bad = ~torch.isfinite(want)
+    assert bool(bad.any())
+    assert torch.equal(torch.nan_to_num(y.double()[bad], nan=0.5, posinf=1.0, neginf=-1.0),
+                       torch.nan_to_num(want[bad], nan=0.5, posinf=1.0, neginf=-1.0))
+    whole = torch.isfinite(x).all(1)
+    if whole.any():
+        _check(x[whole], codes, scales, zeros, group, y[whole])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [1, 8, 9, 20, 64, 70])
+@pytest.mark.parametrize("out_dim,in_dim,group", [(64, 256, 64), (300, 640, 128), (77, 517, 32), (130, 4160, 32)])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_infinities_are_the_definitions(dtype, rows, out_dim, in_dim, group, zeros):
+    codes, scales, zero = _weight(out_dim, in_dim, group, zeros, dtype)
+    if zeros:
+        zero = zero.round()  # zero points that some codes meet: infinity times 0 there
+        zero[::3] = 8.0
+    scales[1] = 0.0
+    x = torch.randn(rows, in_dim, device="cuda").to(dtype)
+    x[-1, in_dim // 2] = torch.inf
+    if rows > 4:
+        x[1, 3] = -torch.inf
+        x[2, in_dim - 1] = torch.nan
+        x[3, 0], x[3, in_dim - 1] = torch.inf, -torch.inf
+    _check_nonfinite(x, codes, scales, zero, group, linear_w4(x, codes, scales, zero, group_size=group))
+
+
+@pytest.mark.parametrize("rows", [2, 20, 64])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_sums_that_only_the_scale_brings_back(rows, zeros):
+    """Activations near the end of bfloat16's range: 7 times them is past float32's, a scale of 0.02 times that is not."""
+    codes, scales, zero = _weight(300, 640, 64, zeros, torch.bfloat16)
+    x = torch.randn(rows, 640, device="cuda").to(torch.bfloat16)
+    x[1, 100] = 2e38
+    y = linear_w4(x, codes, scales, zero, group_size=64)
+    assert torch.isfinite(y).all()
+    _check(x, codes, scales, zero, 64, y)
