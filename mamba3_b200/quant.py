@@ -90,7 +90,7 @@ def linear_w4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros:
 
     On CUDA x is float16 or bfloat16, sums are float32 and the result is rounded once. Meant for
     decoding's few rows (up to 64 share one pass over the weight). Inference only: x must not require
-    grad.
+    grad, on CUDA nor may scales and zeros.
     """
     _validate(x, codes, scales, zeros, group_size)
     if torch.is_grad_enabled() and x.requires_grad:
@@ -102,6 +102,8 @@ def linear_w4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros:
         return F.linear(x.float(), dequantize_w4(codes, scales, zeros, x.shape[-1], group_size=group_size)).to(x.dtype)
     if x.dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"linear_w4 needs float16 or bfloat16 activations on CUDA, got {x.dtype}")
+    if torch.is_grad_enabled() and (scales.requires_grad or zeros is not None and zeros.requires_grad):
+        raise ValueError("linear_w4 is inference only: scales and zeros must not require grad on CUDA")
     if _ext.has_tangent(x, scales, zeros):
         raise ValueError("linear_w4 is inference only: it has no forward-mode derivative on CUDA")
     if scales.dtype not in (torch.float32, torch.float16, torch.bfloat16):

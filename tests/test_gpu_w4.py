@@ -253,3 +253,15 @@ def test_sums_that_only_the_scale_brings_back(rows, zeros):
     y = linear_w4(x, codes, scales, zero, group_size=64)
     assert torch.isfinite(y).all()
     _check(x, codes, scales, zero, 64, y)
+
+
+def test_scales_that_require_grad_are_refused():
+    """The CPU form is differentiable in them; on CUDA the result would have no gradient, without a word."""
+    codes, scales, zero = _weight(16, 64, 64, True, torch.bfloat16)
+    x = torch.randn(2, 64, device="cuda").bfloat16()
+    want = linear_w4(x, codes, scales, zero, group_size=64)
+    for s, z in ((scales.clone().requires_grad_(), zero), (scales, zero.clone().requires_grad_())):
+        with pytest.raises(ValueError, match="inference only"):
+            linear_w4(x, codes, s, z, group_size=64)
+        with torch.no_grad():
+            assert torch.equal(linear_w4(x, codes, s, z, group_size=64), want)
