@@ -71,10 +71,13 @@ class Muon(torch.optim.Optimizer):
         if lr < 0.0 or not 0.0 <= momentum < 1.0 or weight_decay < 0.0:
             raise ValueError("lr and weight_decay must not be negative, momentum must be in [0, 1)")
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps))
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.dim() != 2:
-                    raise ValueError(f"Muon updates matrices; got a parameter of shape {tuple(p.shape)}")
+
+    def add_param_group(self, param_group) -> None:
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() != 2:
+                self.param_groups.pop()
+                raise ValueError(f"Muon updates matrices; got a parameter of shape {tuple(p.shape)}")
 
     @torch.no_grad()
     def step(self, closure=None):

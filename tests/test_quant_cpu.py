@@ -166,3 +166,17 @@ def test_gated_entries_reject_widths_that_overflow():
             assert lib.m3_gated_scan_fwd(_ext._GATED_FORMAT.pack(length, 1, channels, -1, 0, *absent * 14), None) == 1
             assert lib.m3_gated_scan_bwd(_ext._GATED_FORMAT.pack(length, 1, channels, -1, 0, *absent * 14), None) == 1
     assert lib.m3_gated_scan_fwd(_ext._GATED_FORMAT.pack(1, 1, 2 ** 31 - 4097, -1, 0, *absent * 14), None) == 4
+
+
+def test_muon_refuses_vectors_in_groups_added_later():
+    p = torch.nn.Parameter(torch.randn(3, 4))
+    opt = Muon([p])
+    for vector in (torch.nn.Parameter(torch.randn(3)), torch.nn.Parameter(torch.tensor(1.0))):
+        with pytest.raises(ValueError, match="matrices"):
+            opt.add_param_group({"params": [torch.nn.Parameter(torch.randn(2, 2)), vector]})
+    assert len(opt.param_groups) == 1
+    opt.add_param_group({"params": torch.nn.Parameter(torch.randn(2, 5)), "lr": 0.5})
+    for group in opt.param_groups:
+        for q in group["params"]:
+            q.grad = torch.ones_like(q)
+    opt.step()
