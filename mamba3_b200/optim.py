@@ -102,7 +102,7 @@ class Muon(torch.optim.Optimizer):
                 directions = orthogonalize(torch.stack(updates), group["steps"])
                 if group["weight_decay"]:
                     torch._foreach_mul_(params, 1.0 - group["lr"] * group["weight_decay"])
-                scale = math.sqrt(max(1.0, shape[0] / shape[1]))
+                scale = math.sqrt(max(1.0, shape[0] / max(1, shape[1])))
                 torch._foreach_add_(params, [d.to(p.dtype) for d, p in zip(directions.unbind(0), params)],
                                     alpha=-group["lr"] * scale)
         return loss

@@ -180,3 +180,12 @@ def test_muon_refuses_vectors_in_groups_added_later():
         for q in group["params"]:
             q.grad = torch.ones_like(q)
     opt.step()
+
+
+@pytest.mark.parametrize("shape", [(0, 4), (4, 0)])
+def test_muon_passes_empty_matrices_by(shape):
+    empty, p = torch.nn.Parameter(torch.zeros(shape)), torch.nn.Parameter(torch.zeros(2, 3))
+    opt = Muon([empty, p])
+    empty.grad, p.grad = torch.zeros(shape), torch.ones(2, 3)
+    opt.step()
+    assert bool(p.abs().sum() > 0)
