@@ -56,6 +56,10 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, *, coefficients=COEFFICI
     return _ext.orthogonalize(stack, steps, coefficients, out_dtype).view(update.shape)
 
 
+def _wide(p: torch.Tensor) -> torch.dtype:
+    return torch.promote_types(p.dtype, torch.float32)
+
+
 class Muon(torch.optim.Optimizer):
     """Momentum SGD whose update of every matrix is orthogonalised, for the 2-D weights of hidden
     layers (``in_proj`` / ``out_proj``); embeddings, norms and vectors belong to another optimiser.
@@ -63,7 +67,8 @@ class Muon(torch.optim.Optimizer):
         m <- momentum m + grad;  u = orthogonalize(grad + momentum m if nesterov else m)
         w <- w (1 - lr weight_decay) - lr scale u,   scale = sqrt(max(1, rows / cols))
 
-    Matrices of one shape, dtype and device are orthogonalised as one stack.
+    Matrices of one shape, dtype and device are orthogonalised as one stack. The momentum is held in
+    float32 for 16-bit weights too, and u is formed from it there.
     """
 
     def __init__(self, params, lr: float = 0.02, *, momentum: float = 0.95, nesterov: bool = True,
@@ -79,6 +84,14 @@ class Muon(torch.optim.Optimizer):
                 self.param_groups.pop()
                 raise ValueError(f"Muon updates matrices; got a parameter of shape {tuple(p.shape)}")
 
+    def load_state_dict(self, state_dict) -> None:
+        super().load_state_dict(state_dict)  # which casts the momentum to its weight's type
+        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for i, p in zip(saved, (p for group in self.param_groups for p in group["params"])):
+            held = self.state.get(p, {}).get("momentum")
+            if held is not None and held.dtype != _wide(p):
+                self.state[p]["momentum"] = state_dict["state"][i]["momentum"].to(p.device, _wide(p), copy=True)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -91,10 +104,10 @@ class Muon(torch.optim.Optimizer):
                 if p.grad is not None:
                     stacks.setdefault((p.shape, p.dtype, p.device), []).append(p)
             for (shape, _, _), params in stacks.items():
-                grads = [p.grad for p in params]
+                grads = [p.grad.to(_wide(p)) for p in params]
                 for p in params:
                     if "momentum" not in self.state[p]:
-                        self.state[p]["momentum"] = torch.zeros_like(p)
+                        self.state[p]["momentum"] = torch.zeros_like(p, dtype=_wide(p))
                 buffers = [self.state[p]["momentum"] for p in params]
                 torch._foreach_mul_(buffers, group["momentum"])
                 torch._foreach_add_(buffers, grads)

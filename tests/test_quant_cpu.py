@@ -189,3 +189,23 @@ def test_muon_passes_empty_matrices_by(shape):
     empty.grad, p.grad = torch.zeros(shape), torch.ones(2, 3)
     opt.step()
     assert bool(p.abs().sum() > 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_muon_momentum_is_held_in_float32(dtype):
+    """A momentum of 16 bits stands still once a gradient is below its last place: 0.95 m + g with m near 20 g."""
+    torch.manual_seed(0)
+    p = torch.nn.Parameter(torch.randn(3, 4).to(dtype))
+    opt, want = Muon([p], lr=0.0, momentum=0.99), torch.zeros(3, 4, dtype=torch.float64)
+    for step in range(60):
+        p.grad = (0.01 * torch.randn(3, 4, generator=torch.Generator().manual_seed(step)) + 0.1).to(dtype)
+        want = 0.99 * want + p.grad.double()
+        opt.step()
+        if step == 30:  # through a checkpoint
+            other = Muon([torch.nn.Parameter(p.detach().clone())], lr=0.0, momentum=0.99)
+            other.load_state_dict(opt.state_dict())
+            (p,), opt = other.param_groups[0]["params"], other
+    held = opt.state[p]["momentum"]
+    assert held.dtype == torch.float32 and p.dtype == dtype
+    # 60 roundings of 2^-24 of at most the largest value, times 3 for the products
+    assert float((held.double() - want).abs().max()) < 180 * 2.0 ** -24 * float(want.abs().max())
