@@ -60,10 +60,14 @@ def quantize_w4(weight: torch.Tensor, *, group_size: int = 128, zeros: bool = Fa
 def dequantize_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None, in_dim: int, *,
                   group_size: int = 128) -> torch.Tensor:
     """The float32 ``[out, in_dim]`` weight that the codes stand for."""
-    q = torch.stack((codes & 15, codes >> 4), dim=-1).flatten(1)[:, :in_dim].float()
+    return _dequantize(codes, scales, zeros, in_dim, group_size, torch.float32)
+
+
+def _dequantize(codes, scales, zeros, in_dim, group_size, dtype):
+    q = torch.stack((codes & 15, codes >> 4), dim=-1).flatten(1)[:, :in_dim].to(dtype)
     column = torch.arange(in_dim, device=codes.device) // group_size
-    zero = 8.0 if zeros is None else zeros.float()[:, column]
-    return (q - zero) * scales.float()[:, column]
+    zero = 8.0 if zeros is None else zeros.to(dtype)[:, column]
+    return (q - zero) * scales.to(dtype)[:, column]
 
 
 def _validate(x, codes, scales, zeros, group_size) -> None:
@@ -99,7 +103,8 @@ def linear_w4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros:
     if x.numel() == 0 or out_dim == 0:
         return x.new_zeros(*x.shape[:-1], out_dim)
     if not x.is_cuda:
-        return F.linear(x.float(), dequantize_w4(codes, scales, zeros, x.shape[-1], group_size=group_size)).to(x.dtype)
+        wide = torch.promote_types(x.dtype, torch.float32)
+        return F.linear(x.to(wide), _dequantize(codes, scales, zeros, x.shape[-1], group_size, wide)).to(x.dtype)
     if x.dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"linear_w4 needs float16 or bfloat16 activations on CUDA, got {x.dtype}")
     if torch.is_grad_enabled() and (scales.requires_grad or zeros is not None and zeros.requires_grad):

@@ -209,3 +209,14 @@ def test_muon_momentum_is_held_in_float32(dtype):
     assert held.dtype == torch.float32 and p.dtype == dtype
     # 60 roundings of 2^-24 of at most the largest value, times 3 for the products
     assert float((held.double() - want).abs().max()) < 180 * 2.0 ** -24 * float(want.abs().max())
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+def test_float64_products_off_the_gpu(zeros):
+    w = torch.randn(9, 70, dtype=torch.float64)
+    codes, scales, zero = quantize_w4(w, group_size=32, zeros=zeros)
+    x = torch.randn(4, 70, dtype=torch.float64)
+    want = x @ weight_w4(codes, scales, zero, 70, 32).t()
+    torch.testing.assert_close(linear_w4(x, codes, scales, zero, group_size=32), want, rtol=1e-12, atol=1e-12)
+    layer = LinearW4(w, group_size=32, zeros=zeros)
+    torch.testing.assert_close(layer(x), want, rtol=1e-12, atol=1e-12)
