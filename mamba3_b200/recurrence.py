@@ -141,7 +141,7 @@ def gated_scan(value: torch.Tensor, forget: torch.Tensor, gate: torch.Tensor | N
     if value.numel() == 0:
         wide = torch.promote_types(value.dtype, torch.float32)
         state = (torch.zeros(batch, channels, device=value.device, dtype=wide) if initial_state is None
-                 else initial_state.to(wide))
+                 else initial_state.to(wide, copy=True))
         return value.clone(), state
     if not value.is_cuda:
         return _scan_torch(value, forget, gate, initial_state, reset)

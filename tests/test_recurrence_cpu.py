@@ -192,3 +192,13 @@ def test_clusters_have_room(dtype, gate, backward):
             assert cluster == 1 or cluster * batch * -(-channels // 64) <= 148 * room
             sizes.add(cluster)
     assert sizes >= {1, 2, 4, 8}
+
+
+@pytest.mark.parametrize("shape", [(2, 0, 3), (0, 4, 3), (2, 4, 0)])
+def test_the_state_of_an_empty_sequence_is_a_tensor_of_its_own(shape):
+    value, state = torch.empty(shape), torch.randn(shape[0], shape[2])
+    _, final = gated_scan(value, value, initial_state=state)
+    assert torch.equal(final, state)
+    before = state.clone()
+    final.add_(1.0)
+    assert torch.equal(state, before)
