@@ -44,7 +44,7 @@ def quantize_w4(weight: torch.Tensor, *, group_size: int = 128, zeros: bool = Fa
         low, high = w.amin(-1).clamp_max(0.0), w.amax(-1).clamp_min(0.0)
         scales = ((high - low) / 15.0).to(dtype)
         step = torch.where(scales == 0, torch.ones_like(scales), scales).float()
-        zero = (-low / step).to(dtype)
+        zero = (-low / step).clamp_max(15.0).to(dtype)  # past 15 only by the rounding of the scale
         codes = torch.round(w / step[..., None] + zero.float()[..., None])
     else:
         scales = (w.abs().amax(-1) / 7.5).to(dtype)

@@ -220,3 +220,18 @@ def test_float64_products_off_the_gpu(zeros):
     torch.testing.assert_close(linear_w4(x, codes, scales, zero, group_size=32), want, rtol=1e-12, atol=1e-12)
     layer = LinearW4(w, group_size=32, zeros=zeros)
     torch.testing.assert_close(layer(x), want, rtol=1e-12, atol=1e-12)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_zero_points_lie_between_the_codes(dtype):
+    """Negative weights alone put the zero point at 15, where the rounding of the scale must not carry it further: least of
+    all a scale at the end of float16's range, which is half as large again or as small."""
+    for size in (1.0, 0.8, 1.3e-6, 4e-7):
+        w = -size * torch.rand(64, 32, generator=torch.Generator().manual_seed(0))
+        codes, scales, zero = quantize_w4(w, group_size=32, zeros=True, dtype=dtype)
+        assert float(zero.max()) <= 15.0 and float(zero.min()) >= 0.0
+        back = dequantize_w4(codes, scales, zero, 32, group_size=32)
+        # half a step, a step's unit of rounding over 15 codes and the zero point's own; clamped codes of a scale too small
+        scale = scales.float()
+        lost = (-w.amin(1, keepdim=True) - 15.0 * scale).clamp_min(0.0)
+        assert bool(((back - w).abs() <= scale * (0.5 + 15 * 2.0 ** -8) + lost + (scale == 0) * size).all())
