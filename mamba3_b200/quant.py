@@ -140,12 +140,15 @@ class LinearW4(nn.Module):
 
 
 def quantize_projections(model: nn.Module, *, group_size: int = 128, zeros: bool = False) -> nn.Module:
-    """Replace every mixer's ``in_proj`` and ``out_proj`` in ``model`` by 4-bit ones, in place."""
-    for module in list(model.modules()):
-        for name in ("in_proj", "out_proj"):
-            layer = getattr(module, name, None)
-            if isinstance(layer, nn.Linear):
-                if layer.bias is not None:
-                    raise ValueError(f"{name} has a bias: 4-bit projections have none")
-                setattr(module, name, LinearW4(layer.weight, group_size=group_size, zeros=zeros))
+    """Replace every mixer's ``in_proj`` and ``out_proj`` in ``model`` by 4-bit ones, in place (a model
+    that is refused stays as it was)."""
+    found = [(module, name, layer) for module in model.modules() for name in ("in_proj", "out_proj")
+             if isinstance(layer := getattr(module, name, None), nn.Linear)]
+    for _, name, layer in found:
+        if layer.bias is not None:
+            raise ValueError(f"{name} has a bias: 4-bit projections have none")
+    if group_size not in _GROUPS:
+        raise ValueError(f"group_size must be one of {_GROUPS}")
+    for module, name, layer in found:
+        setattr(module, name, LinearW4(layer.weight, group_size=group_size, zeros=zeros))
     return model

@@ -235,3 +235,14 @@ def test_zero_points_lie_between_the_codes(dtype):
         scale = scales.float()
         lost = (-w.amin(1, keepdim=True) - 15.0 * scale).clamp_min(0.0)
         assert bool(((back - w).abs() <= scale * (0.5 + 15 * 2.0 ** -8) + lost + (scale == 0) * size).all())
+
+
+@pytest.mark.parametrize("group", [32, 48])
+def test_a_refused_model_is_left_as_it_was(group):
+    model = GatedRecurrence(64, depth=2)
+    if group == 32:
+        model.layers[1].mixer.out_proj = torch.nn.Linear(128, 64, bias=True)
+    before = {name: type(module) for name, module in model.named_modules()}
+    with pytest.raises(ValueError, match="bias|group_size"):
+        quantize_projections(model, group_size=group)
+    assert {name: type(module) for name, module in model.named_modules()} == before
