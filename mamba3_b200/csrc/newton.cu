@@ -387,7 +387,6 @@ __global__ void __launch_bounds__(Shape<BN, kPair>::kThreads, 1)
   auto acc_empty = [&](int b) { return bars + 8u * (2 * S::kStages + 2 + b); };
   const uint32_t drained = bars + 8u * (2 * S::kStages + 4);
   const uint32_t slot = bars + 8u * (2 * S::kStages + 5);
-  dependents_may_start();
   if (warp == 0 && lane == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&left)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&right)) : "memory");
@@ -410,6 +409,9 @@ __global__ void __launch_bounds__(Shape<BN, kPair>::kThreads, 1)
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(S::kColumns));
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
+    // Only now: the block of a kernel after this one, which waits for this one's end, could otherwise come to this SM
+    // and take the columns first, and both would wait for good.
+    dependents_may_start();
   }
   __syncwarp();
   fence_before();

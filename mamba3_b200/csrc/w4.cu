@@ -492,7 +492,6 @@ __global__ void __launch_bounds__(Many<kN>::kThreads, 1)
   const int slabs = (in_dim + kSlab - 1) / kSlab, per = (slabs + split - 1) / split;
   const int first = min(in_dim, rank * per * kSlab), last = min(in_dim, (rank + 1) * per * kSlab);
   const int stages = (last - first + kStage - 1) / kStage, groups = (last - first + a.group - 1) / a.group;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i)
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(full(i)), "r"(4));
@@ -510,6 +509,9 @@ __global__ void __launch_bounds__(Many<kN>::kThreads, 1)
   if (warp == kProducers / 32) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(M::kColumns));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    // Only now: the block of a kernel after this one, which waits for this one's end, could otherwise come to this SM
+    // and take the columns first, and both would wait for good.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   }
   // Launched as a programmatic dependent: what the kernel before wrote, the weight too if it did, is there only after
   // the wait.

@@ -107,3 +107,17 @@ def test_gemv_rejects_bad_arguments_without_a_device():
     assert lib.m3_gemv(ctypes.byref(args), None) == 1  # more than 4 rows
     args.rows = 1
     assert lib.m3_gemv(ctypes.byref(args), None) != 0  # tensors missing
+
+
+def test_dependents_start_after_tensor_memory_is_allocated():
+    """A kernel that lets the next one start before it has its columns of tensor memory can lose them to the next one's
+    blocks, which then wait for it. Nothing can show that on a GPU but a hang, so the order is read here."""
+    seen = 0
+    for path in sorted((ROOT / "mamba3_b200" / "csrc").glob("*.cu")):
+        for body in path.read_text().split("__global__")[1:]:
+            body = body[:body.index("\n}\n")]
+            starts = [body.find(word) for word in ("griddepcontrol.launch_dependents", "dependents_may_start();") if word in body]
+            if starts and "tcgen05.alloc" in body:
+                seen += 1
+                assert min(starts) > body.rindex("tcgen05.alloc"), path.name
+    assert seen == 2
