@@ -237,6 +237,9 @@ typedef struct m3_orth_args {
 } m3_orth_args;
 
 int64_t m3_orthogonalize_workspace_bytes(const m3_orth_args* args);
+/* Width of the tiles that a call's products take: 256 (a pair of CTAs a tile), 128 or 64; product 0 is X X^T, 1 A A, 2 P X.
+   Launches nothing. */
+int m3_orthogonalize_tile(const m3_orth_args* args, int product);
 int m3_orthogonalize(const m3_orth_args* args, void* stream);
 
 /* Chunked SSD forward. Returns M3_OK or an M3_ERR_* code. */

@@ -173,6 +173,8 @@ def load() -> ctypes.CDLL:
             getattr(lib, name).restype = ctypes.c_int
         lib.m3_orthogonalize_workspace_bytes.argtypes = [ctypes.c_char_p]
         lib.m3_orthogonalize_workspace_bytes.restype = ctypes.c_int64
+        lib.m3_orthogonalize_tile.argtypes = [ctypes.c_char_p, ctypes.c_int]
+        lib.m3_orthogonalize_tile.restype = ctypes.c_int
         if lib.m3_abi_version() != ABI_VERSION:
             raise RuntimeError("mamba3_b200 library ABI mismatch; rebuild it")
         _lib = lib

@@ -763,11 +763,17 @@ cudaError_t launch_product(Product p, const Stack& left, const Stack& right, int
 
 // The widest tile whose tiles still occupy half of the SMs: wide tiles read less from L2 for each product,
 // narrow ones keep small stacks off a few SMs.
+int tile_width(const Product& p, int count) {
+  return 4 * tile_count(p, 256, 256, count) >= sm_count() ? 256 : 2 * tile_count(p, 128, 128, count) >= sm_count() ? 128 : 64;
+}
+
 template <bool kRightByRows>
 cudaError_t launch(const Product& p, const Stack& left, const Stack& right, int count, cudaStream_t stream) {
-  if (4 * tile_count(p, 256, 256, count) >= sm_count()) return launch_product<256, kRightByRows, true>(p, left, right, count, stream);
-  if (2 * tile_count(p, 128, 128, count) >= sm_count()) return launch_product<128, kRightByRows, false>(p, left, right, count, stream);
-  return launch_product<64, kRightByRows, false>(p, left, right, count, stream);
+  switch (tile_width(p, count)) {
+    case 256: return launch_product<256, kRightByRows, true>(p, left, right, count, stream);
+    case 128: return launch_product<128, kRightByRows, false>(p, left, right, count, stream);
+    default: return launch_product<64, kRightByRows, false>(p, left, right, count, stream);
+  }
 }
 
 cudaError_t run(const m3_orth_args& a, cudaStream_t stream) {
@@ -863,6 +869,16 @@ extern "C" int64_t m3_orthogonalize_workspace_bytes(const m3_orth_args* args) {
   if (args == nullptr) return -report_error(M3_ERR_ARGUMENT, "null argument struct");
   const int rc = newton::check(*args);
   return rc != M3_OK ? -rc : newton::plan(*args).bytes;
+}
+
+extern "C" int m3_orthogonalize_tile(const m3_orth_args* args, int product) {
+  using namespace m3;
+  if (args == nullptr || newton::check(*args) != M3_OK) return 0;
+  newton::Product p = {};
+  p.m = (int)std::min(args->rows, args->cols);
+  p.n = product == 2 ? (int)std::max(args->rows, args->cols) : p.m;
+  p.symmetric = product != 2;
+  return newton::tile_width(p, args->count);
 }
 
 extern "C" int m3_orthogonalize(const m3_orth_args* args, void* stream) {

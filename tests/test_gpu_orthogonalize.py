@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from _operator_refs import orthogonalize64
-from mamba3_b200 import GatedRecurrence, Muon, orthogonalize
+from mamba3_b200 import GatedRecurrence, Muon, _ext, orthogonalize
 from mamba3_b200.optim import COEFFICIENTS
 
 pytestmark = pytest.mark.gpu
@@ -132,3 +132,51 @@ def test_muon_steps_are_the_formula_and_lower_the_loss():
             moved = (w.double() * (1 - 0.02 * 0.01) - p.detach().double()) / scale
             assert _off(moved, orthogonalize64(p.grad + 0.9 * m, 5, COEFFICIENTS)) < BOUND
     assert losses[-1] < losses[0]
+
+
+def _widths(count, rows, cols):
+    args = _ext._ORTH_FORMAT.pack(rows, cols, count, 5, 0, 1.0, 1.0, 1.0, *_ext._ABSENT * 3)
+    return tuple(_ext.load().m3_orthogonalize_tile(args, product) for product in range(3))
+
+
+def _iterate64(u, steps, coefficients):
+    """The definition in float64 products on the GPU, where the singular values take the CPU too long."""
+    a, b, c = coefficients
+    x = u.double()
+    x = x.mT if u.shape[-2] > u.shape[-1] else x
+    x = x / torch.linalg.matrix_norm(x, keepdim=True)
+    for _ in range(steps):
+        gram = x @ x.mT
+        x = a * x + (b * gram + c * gram @ gram) @ x
+    return x.mT if u.shape[-2] > u.shape[-1] else x
+
+
+# stacks of matrices, and the tiles of X X^T, A A and P X on 148 SMs: pairs of CTAs (256), single ones with 128 or 64 columns.
+# Only pairs ever have more tiles than places (74): 16 x 520 x 1030, 8 x 1030 x 1100 and the last three have.
+TILES = [((1, 1100, 1300), (64, 64, 128)), ((4, 500, 700), (64, 64, 128)), ((4, 700, 900), (128, 128, 256)),
+         ((5, 650, 660), (128, 128, 256)), ((1, 1030, 2100), (64, 64, 256)), ((1, 2100, 1030), (64, 64, 256)),
+         ((2, 1270, 1280), (128, 128, 256)), ((16, 520, 1030), (256, 256, 256)), ((8, 1030, 1100), (256, 256, 256)),
+         ((1, 2305, 2561), (256, 256, 256)), ((3, 2561, 1793), (256, 256, 256)), ((1, 3333, 3077), (256, 256, 256))]
+
+
+@pytest.mark.parametrize("shape,widths", TILES)
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_every_tile_of_the_products(shape, widths, out_dtype):
+    assert _widths(*shape) == widths
+    for dtype in (torch.float32, torch.bfloat16):
+        u = _update(*shape, dtype, seed=shape[1])
+        got = orthogonalize(u, out_dtype=out_dtype)
+        want = _iterate64(u, 5, COEFFICIENTS)
+        assert got.dtype == out_dtype
+        for g, w in zip(got, want):
+            assert _off(g, w) < BOUND
+            # no element far from its own: an error of a tile or a triangle would be of the size of the entries
+            assert float((g.double() - w).abs().max()) < 0.1 * float(w.abs().max())
+
+
+@pytest.mark.parametrize("shape", [(8, 1030, 1100), (4, 700, 900), (1, 1100, 1300)])
+def test_products_repeat_bitwise(shape):
+    u = _update(*shape)
+    first = orthogonalize(u, out_dtype=torch.float32)
+    for _ in range(5):
+        assert torch.equal(orthogonalize(u, out_dtype=torch.float32), first)
