@@ -754,46 +754,50 @@ template <typename T, bool kGate, bool kBackward> struct Pass {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem(kMaxCluster));
     return e != cudaSuccess ? e : cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   }
-  // Clusters of 16 that the device hosts at once where an SM has room for one of their CTAs only; 0 without a device.
-  static int hosted() {
-    static std::atomic<int> cached[64];
+  // Clusters of `size` that the device hosts at once, as it says itself: a cluster lies within a group of 16 to 20 SMs,
+  // and what is left of a group holds none. Without a device, 148 SMs without groups.
+  static int64_t hosted(int size) {
+    static std::atomic<int> cached[64][kMaxCluster + 1];
     int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
-      cudaGetLastError();
-      return 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64) {
+      std::atomic<int>& held = cached[dev][size];
+      if (const int known = held.load(std::memory_order_relaxed)) return known - 1;
+      const auto kernel = pass_kernel<T, kGate, true, kBackward>();
+      cudaLaunchAttribute attr[1];
+      const cudaLaunchConfig_t cfg = config(dim3(size), size, attr, nullptr);
+      if (raise_limits(kernel) == cudaSuccess && cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess) {
+        held.store(n + 1, std::memory_order_relaxed);
+        return n;
+      }
     }
-    if (const int held = cached[dev].load(std::memory_order_relaxed)) return held - 1;
-    const auto kernel = pass_kernel<T, kGate, true, kBackward>();
-    cudaLaunchAttribute attr[1];
-    const cudaLaunchConfig_t cfg = config(dim3(kMaxCluster), kMaxCluster, attr, nullptr);
-    if (raise_limits(kernel) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
-      cudaGetLastError();
-      return 0;
-    }
-    cached[dev].store(n + 1, std::memory_order_relaxed);
-    return n;
+    cudaGetLastError();
+    return size > 8 && room(size) < 2 ? 0 : (int64_t)sm_count() * room(size) / size;
   }
 };
 
 template <typename P> int cluster_size(const m3_gated_args& a) {
   const int64_t ntiles = (a.length + kTile - 1) / kTile;
   const int64_t blocks = (int64_t)a.batch * ((a.channels + kChannels - 1) / kChannels);
-  // A cluster takes a sequence's tiles together while its CTAs still have room on the GPU at once: clusters of up to
-  // 4 in all the room there is (4 x 2048 x 2048: 47 us in fours, 54 in twos), larger ones, whose exchange takes as long
-  // as a tile, up to two CTAs an SM (1 x 65536 x 1536: 308 us in eights, 328 in sixteens; 1 x 32768 x 128: 83 us in
-  // sixteens, 136 in eights), and tens where sixteens have no such room (1 x 65536 x 1536: 267 us, backward 647 against
-  // 762). Where the CTAs of eights have all their tiles under way from the start, they take all the room too
-  // (3 x 777 x 1001: 17 us, 26 in fours). Past 8 CTAs, a cluster's size without conditions, only where two fit an SM; or
-  // sixteens where the device has SMs enough side by side for all of them (float32 with a gate, whose sixteens fit one
-  // an SM: 1 x 32768 x 128 in 80 us, 117 in tens; 1 x 65536 x 1024, 16 clusters that it has not: 438 us, 295 in tens).
+  // A cluster takes a sequence's tiles together while the device hosts all clusters at once: clusters of up to 4 in all the
+  // room there is, larger ones, whose exchange takes as long as a tile, up to two CTAs an SM, and eights, where all their
+  // tiles are under way from the start, in all the room too. Sixteens are the last power; tens stand where sixteens have no
+  // such room. Measured in bf16 with a gate, forward and backward, us:
+  //                                          2           4           8          10          16
+  //   1 x 65536 x 1216   (19 x 64 channels)  932, 2060   472, 1060   294, 686   255, 578    203, 650
+  //   1 x 65536 x 1536   (24)                933, 2072   473, 1064   298, 691   256, 583    318, 736
+  //   1 x 65536 x 1856   (29)                933, 2076   473, 1071   303, 699   310, 1006   351, 995
+  //   2 x 4096 x 1024    (32)                61.7, 133   32.8, 72.9  23.2, 48.9 24.7, 74.2  28.1, 71.4
+  //   4 x 2048 x 1024    (64)                32.5, 69.0  22.0, 47.4  27.6, 51.7 27.6, 70.3  30.9, 71.4
+  //   1 x 640 x 4736     (74)                12.5, 23.3  12.2, 31.0  16.4, 35.3 12.4, 25.1
+  //   3 x 777 x 1001, float32, no gate (48)  34.1, 39.6  23.7, 32.1  16.7, 32.6 27.9, 66.8
+  // What is not hosted at once runs in waves: tens of 29 (backward), fours of 74 (backward, 296 CTAs for 296 places).
   int cluster = 1;
   for (int size = 2; size <= kMaxCluster && size <= ntiles; size *= 2) {
     const bool all_room = size < 8 || (size == 8 && 8 * kStages >= ntiles);
-    if (size * blocks > (int64_t)sm_count() * (all_room ? P::room(size) : std::min(P::room(size), 2))) break;
-    if (size > 8 && P::room(size) < 2 && blocks > P::hosted()) break;
+    if (blocks > P::hosted(size) || (!all_room && size * blocks > 2 * (int64_t)sm_count())) break;
     cluster = size;
   }
-  if (cluster == 8 && P::room(10) >= 2 && 10 <= ntiles && 10 * blocks <= 2 * (int64_t)sm_count()) cluster = 10;
+  if (cluster == 8 && P::room(10) >= 2 && 10 <= ntiles && 10 * blocks <= 2 * (int64_t)sm_count() && blocks <= P::hosted(10)) cluster = 10;
   return cluster;
 }
 
