@@ -43,7 +43,7 @@ using umma::tma_load3;
 
 constexpr int kTile = 64;        // tokens a tile: the training forward keeps the state before each
 constexpr int kChannels = 64;    // channels a CTA; a thread has two neighbouring ones
-constexpr float kFloor = 1e-37f; // least product of decays without a reset: see fold()
+constexpr float kFloor = 1.4013e-45f;  // least product of decays without a reset, float32's least number: see fold()
 
 template <typename T> constexpr bool kFine = std::is_same<T, float>::value;
 
@@ -78,14 +78,18 @@ __device__ __forceinline__ float at_most(float x, float most) {
   return x;
 }
 
-// f = sigmoid(x) and 1 - f = sigmoid(-x); x below -80 is taken as -80 (f = 2e-35), so that exp stays finite; NaN stays
-// NaN. (kExact: past 100, where exp(-x) is 0, the differences of infinities are kept out.)
+// f = sigmoid(x) and 1 - f = sigmoid(-x). exp(-x) is kept at 2^125 or less, so that its reciprocal is no subnormal number
+// (x at -125 ln 2 = -86.6 or more), and what f is there, 2^-125, is taken off every f: a masked logit (the type's lowest
+// value, an infinity) drops a state of any size, and f is itself wherever it is not below 2^-100. NaN stays NaN.
+// (kExact: past 100, where exp(-x) is 0, the differences of infinities are kept out.)
 template <bool kExact> __device__ __forceinline__ void keep_lose(float x, float& keep, float& lose) {
-  float c = at_least(x, -80.0f);
-  if (kExact) c = at_most(c, 100.0f);
-  const float e = exp_minus<kExact>(c);
-  keep = reciprocal<kExact>(1.0f + e);
-  lose = e * keep;
+  constexpr float kLeast = -86.643394f, kAtLeast = kExact ? 2.3509960e-38f /* exp(kLeast) */ : 2.3509887e-38f /* 2^-125 */;
+  float e;
+  if constexpr (kExact) e = exp_minus<true>(at_most(at_least(x, kLeast), 100.0f));
+  else e = ex2_approx(at_most(x * -kLog2e, 125.0f));
+  const float f = reciprocal<kExact>(1.0f + e);
+  keep = f - kAtLeast;
+  lose = e * f;
 }
 
 // sigmoid(x), 0 below -88.

@@ -354,3 +354,36 @@ def test_every_split_of_a_float32_sequence(length, channels, gated):
                       gated_scan64)
     for i, (a, e) in enumerate(zip(got, want)):
         assert_rounded(a, e, 2 * SUMS, f"gradient {i}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("length", [1, 40, 700])
+def test_masks_of_the_lowest_value(dtype, length):
+    """Padding whose value is the type's lowest, before tokens whose forget logit drops the state: -inf, the lowest value,
+    or -200, where float32's sigmoid is 0; and a state of that size from before. Nothing of it may be left."""
+    lowest = torch.finfo(dtype).min
+    for masked in (-torch.inf, lowest, -200.0):
+        value, forget, gate, state, _ = _inputs(2, length, 70, dtype)
+        first = torch.arange(length, device="cuda") % 23 == 0
+        forget[:, first] = masked
+        state[:] = torch.finfo(torch.float32).min
+        value[:, torch.arange(length, device="cuda") % 23 == 22] = lowest
+        y, final = gated_scan(value, forget, gate, initial_state=state)
+        want_y, want_final = gated_scan64(value, forget, gate, state)
+        padded = torch.arange(length, device="cuda") % 23 == 22
+        assert_rounded(y[:, ~padded], want_y[:, ~padded], SUMS, "y")  # without the values that are as large as the mask
+        if not padded[-1]:
+            assert_rounded(final, want_final, SUMS, "state")
+        if length == 1:
+            y, new = gated_step(value[:, 0], forget[:, 0], state, gate[:, 0])
+            assert_rounded(y, want_y[:, 0], SUMS)
+            assert_rounded(new, want_final, SUMS)
+        dy, dstate = torch.randn_like(value), torch.randn_like(state)
+        got = _gradients(value, forget, gate, state, None, dy, dstate,
+                         lambda v, f, q, s, r: gated_scan(v, f, q, initial_state=s, reset=r))
+        want = _gradients(value.double(), forget.double(), gate.double(), state.double(), None, dy, dstate, gated_scan64)
+        for name, a, e in zip(("value", "forget", "gate", "state"), got, want):
+            if name == "value":
+                assert_rounded(a, e, 2 * SUMS, name)
+            elif name == "state":  # f is within 4 of float32's least numbers, 5.6e-45, and the gradients after it below 1e4
+                assert float(a.abs().max()) <= 1e-40
