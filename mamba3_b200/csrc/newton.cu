@@ -27,15 +27,7 @@ namespace m3 {
 int report_error(int code, const char* msg);
 
 // The error word of this unit's bounded waits, for m3_device_error(); the device is synchronised.
-int read_newton_error(int clear) {
-  int host = 0;
-  if (cudaMemcpyFromSymbol(&host, g_device_error, sizeof(int)) != cudaSuccess) return -1;
-  if (clear) {
-    const int zero = 0;
-    if (cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int)) != cudaSuccess) return -1;
-  }
-  return host;
-}
+int read_newton_error(int clear) { return read_unit_error(clear); }
 
 namespace newton {
 

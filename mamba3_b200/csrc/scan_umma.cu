@@ -43,14 +43,7 @@
 namespace m3 {
 
 int read_device_error(int clear) {
-  int host = 0;
-  if (cudaDeviceSynchronize() != cudaSuccess) return -1;
-  if (cudaMemcpyFromSymbol(&host, g_device_error, sizeof(int)) != cudaSuccess) return -1;
-  if (clear) {
-    const int zero = 0;
-    if (cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int)) != cudaSuccess) return -1;
-  }
-  return host;
+  return cudaDeviceSynchronize() != cudaSuccess ? -1 : read_unit_error(clear);
 }
 
 namespace umma {

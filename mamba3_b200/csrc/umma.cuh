@@ -15,6 +15,17 @@ namespace m3 {
 // reads every unit's).
 static __device__ int g_device_error = 0;
 
+// This unit's error word; the device is synchronised.
+static inline int read_unit_error(int clear) {
+  int host = 0;
+  if (cudaMemcpyFromSymbol(&host, g_device_error, sizeof(int)) != cudaSuccess) return -1;
+  if (clear) {
+    const int zero = 0;
+    if (cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int)) != cudaSuccess) return -1;
+  }
+  return host;
+}
+
 inline int sm_count() {
   static int cached[64] = {};
   int dev = 0;
