@@ -183,8 +183,7 @@ int m3_gemv(const m3_gemv_args* args, void* stream);
  *         of m3_gated_tile() tokens, written by the forward when given and read by the backward
  * Backward (m3_gated_scan_bwd, with the forward's inputs and carry): dy [B,L,C] and dstate [B,C]
  * float32 (optional, the gradient of out_state) give dvalue, dforget, dgate [B,L,C] and, when given,
- * dinitial [B,C] float32. The reference has no such recurrence; it stands beside the SSD scan in
- * stacks that mix the two.
+ * dinitial [B,C] float32. The reference has no such recurrence. At most 2^31 - 4097 channels.
  */
 typedef struct m3_gated_args {
   int64_t length;
@@ -225,7 +224,8 @@ int m3_linear_w4(const m3_w4_args* args, void* stream);
  * and strides): X_0 = G / |G|_F (0 where G = 0), then `steps` times
  *   A = X X^T,  X <- a X + (b A + c A A) X      (on the transpose where rows > cols),
  * coefficient = {a, b, c}; out [count][rows][cols] is X in out's float dtype. The caller passes
- * workspace: m3_orthogonalize_workspace_bytes(args) bytes, 256-byte aligned. No counterpart in the
+ * workspace: m3_orthogonalize_workspace_bytes(args) bytes, 256-byte aligned. Products take 16-bit
+ * operands and float32 sums; entries of an iterate or of A must stay below 255. No counterpart in the
  * reference, which has no optimiser.
  */
 typedef struct m3_orth_args {

@@ -368,10 +368,11 @@ __device__ __forceinline__ float4 open_run(const T* forget, const T* value, int 
 // out of registers. CTAs walk a sequence's tiles one after another; where sequences and channels are too few to
 // fill the GPU, a cluster walks them together. Every input is read once and nothing but y, the last state and, for a
 // backward pass, a state a tile is written.
-// bf16 with a gate: 8 x 8192 x 2048 in 230 us (4.7 TB/s, 72 % of a copy), 4 x 2048 x 2048 in 46 (49 with the states
-// kept), 1 x 65536 x 1536 in 256. Full grids are bound by issue slots, IPC 2 with the special-function unit (two
-// exp2 and two reciprocals a value) half used; few channels by the exchange of a cluster's maps, step after step. Runs
-// of 16 tokens halve the folding that runs of 8 need.
+// bf16 with a gate: 8 x 8192 x 2048 in 227 us (4.7 TB/s, 73 % of a copy), 4 x 2048 x 2048 in 39, 1 x 65536 x 1536 in 264.
+// On full grids nothing is at its limit: 128 registers a thread leave sixteen warps an SM, whose chains of dependent
+// instructions fill 56 % of the issue slots, the special-function unit (two exp2 and two reciprocals a value) half and
+// DRAM's rate to 36 % (4 x 2048 x 2048). Few channels wait for the exchange of a cluster's maps, step after step. Runs of
+// 16 tokens halve the folding that runs of 8 need.
 constexpr int kFwdWarps = 4, kFwdThreads = 32 * kFwdWarps, kFwdRun = kTile / kFwdWarps;
 
 template <typename T, bool kGate, bool kVec>
@@ -464,9 +465,10 @@ __global__ void __launch_bounds__(kFwdThreads, 4)
 
 // Backward, the tiles from the last to the first: the states of a tile come from the state kept before it, as in
 // the forward, and the gradients In run back through maps of the same a with h0 of their own.
-// bf16 with a gate: 8 x 8192 x 2048 in 592 us (3.2 TB/s, 49 % of a copy), 4 x 2048 x 2048 in 107, 1 x 65536 x 1536 in
-// 611. Bound by issue: five pairs of values a token are held over the tile's barrier, 128 registers a thread for runs of
-// 8, so four warps a scheduler, IPC 2.2. Runs of 4 in 16 warps of 64 registers: 1002 us; of 16 in four warps, slower too.
+// bf16 with a gate: 8 x 8192 x 2048 in 577 us (3.3 TB/s, 50 % of a copy), 4 x 2048 x 2048 in 92, 1 x 65536 x 1536 in
+// 590. Five pairs of values a token are held over the tile's barrier, 128 registers a thread for runs of 8, so four warps
+// a scheduler: 57 % of the issue slots, DRAM's rate to 27 %, no pipe above 36 % (4 x 2048 x 2048); a warp waits most for
+// the instruction before. Runs of 4 in 16 warps of 64 registers: 1002 us against 650 then; of 16 in four warps, slower too.
 constexpr int kBwdWarps = 8, kBwdThreads = 32 * kBwdWarps, kBwdRun = kTile / kBwdWarps;
 
 template <typename T, bool kGate, bool kVec>

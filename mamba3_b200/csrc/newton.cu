@@ -360,9 +360,13 @@ __device__ __forceinline__ void pair_commit(uint32_t bar) {
 // instruction touches 32 lines, and a 128 x 256 tile took longer to store (7 us) than its MMAs at k = 2560.
 // A block is a chain of latencies (about 3000 clocks), so sixteen warps share a tile's: with four, and TMA loads
 // and stores of the boxes to wait for, a tile took 8 us.
-// 10768 x 2560, five steps: 1251 us, 913 TFLOP/s of the products that symmetry leaves, at the 1.55 GHz that the power
-// limit allows; a K step of 16 takes 133 clocks of 128. 128 x 256 tiles of single CTAs took 1490 us. 4 x 1336 x 256:
-// 127 us, fifteen products of about 7 us each, bound by the launches that wait for one another.
+// 10768 x 2560, five steps: 1242 us, 920 TFLOP/s of the products that symmetry leaves; a step's X X^T takes 78 us, its
+// A A 31 and its P X 120 in the loop. P X (430 tiles on 74 pairs, six waves) has 960 K steps of 16 a pair, 128 clocks each
+// of the tensor pipe, and takes 186 thousand clocks, at 1.54 GHz: the pipe is busy 64 % of the time. A step takes 133
+// clocks once a tile is under way; first loads and the last tile's epilogue take about 16 thousand, and where the rest
+// goes has not been found. X X^T and A A have one wave on 55 of the 74 pairs (pipe 52 and 29 % of the time; A A's epilogue
+// is as long as its K steps). 128 x 256 tiles of single CTAs took 1490 us against 1298. 4 x 1336 x 256: 128 us,
+// fifteen products of about 7 us each, bound by the launches that wait for one another.
 template <int BN, bool kRightByRows, bool kPair>
 __global__ void __launch_bounds__(Shape<BN, kPair>::kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__ CUtensorMap right, const Product p) {
@@ -754,7 +758,17 @@ cudaError_t launch_product(Product p, const Stack& left, const Stack& right, int
 }
 
 // The widest tile whose tiles still occupy half of the SMs: wide tiles read less from L2 for each product,
-// narrow ones keep small stacks off a few SMs.
+// narrow ones keep small stacks off a few SMs. us with the symmetric products / P X in tiles of
+//                      64 / 64   64 / 128  64 / 256  128 / 128  128 / 256  256 / 256   the rule's
+//   10768 x 2560       2412      1856      1607      1652       1501       1168        256 / 256
+//   2048 x 2048        456       372       348       301        275        332         128 / 256
+//   8 x 512 x 2048     310       301       296       263        258        303         128 / 256
+//   2 x 1024 x 4096    383       325       309       345        328        374         64 / 256
+//   1336 x 1336        198       175       199       195        214        261         64 / 128
+//   4 x 1336 x 256     124       121       144       140        162        197         64 / 128
+//   16 x 256 x 256     99        108       127       122        144        178         64 / 64
+//   4 x 1024 x 2048    434       358       338       307        288        344         256 / 256: not the best
+//   4 x 700 x 900      180       182       183       200        198        242         128 / 256: not the best
 int tile_width(const Product& p, int count) {
   return 4 * tile_count(p, 256, 256, count) >= sm_count() ? 256 : 2 * tile_count(p, 128, 128, count) >= sm_count() ? 128 : 64;
 }

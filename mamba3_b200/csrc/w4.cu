@@ -6,7 +6,8 @@
 // What bounds it is the stream of the codes, O I / 2 bytes, and their conversion on the way: at the copy rate an SM has
 // about 2.7 instructions of a lane for a code, a conversion to float32 and a multiply-add take as many. So the
 // products go to the warp-level tensor instruction (m16n8k16: 16 outputs x 8 rows of x), whose 16-bit operands take
-// two codes at a time: bits of (1024 + code) less 1032 is code - 8 exactly (in bf16: 128 and 136). Which column goes
+// two codes at a time: bits of (1024 + code) less 1032 is code - 8 exactly (in bf16: 128 and 136; the use of an exponent's
+// free bits for this is Kim, Henry, Fahim and Awadalla's, 2022). Which column goes
 // where in a product is free as long as both operands agree, so the codes are used as they lie in memory: four
 // threads share an output row, and of every group a thread has group / 4 neighbouring columns, one load of 4, 8 or
 // 16 bytes. Products of 16-bit values by code - 8 are exact, sums float32, scaled group by group:
@@ -269,8 +270,10 @@ __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466
 // ---- up to 8 rows --------------------------------------------------------------------------------
 // A stream of codes: one CTA for 16 outputs, its warps share the columns out, slab by slab, and meet in shared memory.
 // x, a few KB, comes from L1 as the products want it. 10768 x 2560, groups of 128: 6.3 us at one row (2.2 TB/s of codes),
-// 7.1 at eight, groups of 64 and 32: 7.7 and 9.5; 8192 x 8192: 17.8; what bounds it at these sizes is a wave's latency,
-// the launch, the first codes and the meeting of the warps. Scales widened where they are fetched cost 1.6 us of 8.
+// 7.1 at eight, groups of 64 and 32: 7.7 and 9.5: one wave of CTAs, twenty warps an SM, whose time is the launch, the
+// first codes and the meeting of the warps. 8192 x 8192: 17.8, 512 CTAs of sixteen warps, of which the registers allow
+// one an SM, so four waves, each warp waiting for its two slabs of codes and for x (five of nine clocks a warp between
+// instructions; 40 % of the issue slots, DRAM's rate to 21 %). Scales widened where they are fetched cost 1.6 us of 8.
 // Rows of codes that are no whole words (10768 x 2561): 21.
 constexpr int kMostWarps = 16;
 

@@ -141,7 +141,11 @@ class LinearW4(nn.Module):
 
 def quantize_projections(model: nn.Module, *, group_size: int = 128, zeros: bool = False) -> nn.Module:
     """Replace every mixer's ``in_proj`` and ``out_proj`` in ``model`` by 4-bit ones, in place (a model
-    that is refused stays as it was)."""
+    that is refused stays as it was).
+
+    The model is for inference from then on: run it under ``torch.no_grad()`` or ``inference_mode()``.
+    In grad mode its ``forward`` raises, since a norm's weight requires grad and so do the projections'
+    inputs. Scales and zero points take the weight's type."""
     found = [(module, name, layer) for module in model.modules() for name in ("in_proj", "out_proj")
              if isinstance(layer := getattr(module, name, None), nn.Linear)]
     for _, name, layer in found:

@@ -3,8 +3,8 @@
     f_t = sigmoid(forget_t);  h_t = f_t h_{t-1} + (1 - f_t) value_t;  y_t = h_t silu(gate_t)
 
 per (batch, channel). :func:`gated_scan` runs whole sequences (differentiable), :func:`gated_step`
-one token; :class:`GatedRecurrence` is a shape-preserving stack with the call surface of ``Mamba3``
-(``forward``, ``prefill``, ``step``, and ``GatedRecurrence.step`` is CUDA-graph capturable).
+one token; :class:`GatedRecurrence` is a shape-preserving stack with ``forward``, ``prefill`` and
+``step`` as ``Mamba3`` has them (``step`` can be captured in a CUDA graph).
 
 Dispatch follows :mod:`mamba3_b200.ops`: CUDA tensors run the kernels of ``csrc/gated.cu`` (forward
 and backward), with no other GPU path; CPU tensors run the PyTorch formulation below.
@@ -133,7 +133,8 @@ def gated_scan(value: torch.Tensor, forget: torch.Tensor, gate: torch.Tensor | N
     (float32, float16 or bfloat16), of any strides: columns of one projection are read in place.
     On CUDA it has gradients in reverse mode, once; forward mode is refused.
     ``initial_state`` is ``[B, C]`` float32 (zeros without it). ``reset`` ``[B, L]`` (bool) marks
-    tokens that start a document: they see a zero state. The state is held in float32; ``y`` and the
+    tokens that start a document: they see a zero state, whatever it held. (A forget logit of -inf, or
+    the type's lowest value, drops a finite state too.) The state is held in float32; ``y`` and the
     gradients are rounded once, to the inputs' dtype.
     """
     _validate(value, forget, gate, initial_state, reset)
@@ -244,11 +245,12 @@ class _GatedBlock(nn.Module):
 
 class GatedRecurrence(nn.Module):
     """A shape-preserving stack of gated-recurrence mixers, ``[batch, length, d_model]`` in and out:
-    RMSNorm -> mixer -> residual per block, RMSNorm at the end, the surface of ``Mamba3``.
+    RMSNorm -> mixer -> residual per block, RMSNorm at the end. It has no ``cuda_graph`` and no chunk
+    sizes, and ``prefill`` starts from zero states.
 
     ``forward(x, reset=None)`` is differentiable; ``prefill(x)`` also returns the decode cache (one
     float32 ``[batch, 2 * d_model]`` state per layer); ``step(x, cache)`` processes one token, in place
-    in the cache with ``in_place=True``.
+    in the cache with ``in_place=True`` (on CUDA without gradients).
     """
 
     def __init__(self, d_model: int, depth: int = 4) -> None:
