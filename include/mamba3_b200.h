@@ -206,8 +206,8 @@ int m3_gated_scan_bwd(const m3_gated_args* args, void* stream);
  *   x [rows][in_dim], y [rows][out_dim]   one 16-bit dtype
  *   codes [out_dim][(in_dim + 1) / 2]     bytes (M3_U8), the even column in a byte's low half
  *   scales, zeros [out_dim][ceil(in_dim / group)]  one float dtype; zeros optional (8 everywhere)
- * group 32, 64 or 128. Float32 sums, y rounded once. Any strides; rows of 16-byte-aligned contiguous
- * bytes are the fast layout. No counterpart in the reference, whose projections are 16- or 32-bit.
+ * group 32, 64 or 128. Float32 sums, y rounded once; a sum that is not finite is taken again term by term.
+ * At most 64 * 65535 rows. Any strides; rows of 16-byte-aligned contiguous bytes are the fast layout. No counterpart in the reference, whose projections are 16- or 32-bit.
  */
 typedef struct m3_w4_args {
   int64_t out_dim, in_dim;
@@ -225,8 +225,8 @@ int m3_linear_w4(const m3_w4_args* args, void* stream);
  *   A = X X^T,  X <- a X + (b A + c A A) X      (on the transpose where rows > cols),
  * coefficient = {a, b, c}; out [count][rows][cols] is X in out's float dtype. The caller passes
  * workspace: m3_orthogonalize_workspace_bytes(args) bytes, 256-byte aligned. Products take 16-bit
- * operands and float32 sums; entries of an iterate or of A must stay below 255. No counterpart in the
- * reference, which has no optimiser.
+ * operands and float32 sums; entries of an iterate or of A must stay below 255. At most 65535 matrices,
+ * of at most 65536 x 1048576. No counterpart in the reference, which has no optimiser.
  */
 typedef struct m3_orth_args {
   int64_t rows, cols;
