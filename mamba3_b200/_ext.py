@@ -504,8 +504,9 @@ def gemv(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
 def has_tangent(*tensors) -> bool:
     """Whether a tensor carries a tangent of ``torch.autograd.forward_ad``. Such a dual tensor has ``requires_grad``
     False and data like any other's; a kernel that runs on it gives a result without a tangent, a derivative of 0."""
-    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
-                                                  for t in tensors)
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no level is open; asking each tensor costs a microsecond
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 # ---- operators whose argument structs are packed in one go -----------------------------------------
